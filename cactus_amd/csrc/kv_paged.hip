@@ -1,0 +1,332 @@
+// The paged INT8 key/value cache (include/cactus_hip_paged.h): appending the rows of a step, reading tokens back.
+//
+// Append.  k' = rope(rms_norm(k)), q' = rope(rms_norm(q)); the page's scale of k' (and of v) is the running
+// max(|x|) / 127 of its tokens, q = rne(x / scale).  Bound: HBM for prompts (rows in, INT8 and the q rows out: every byte
+// moves once), launch latency for a decode step.
+//
+// A workgroup takes the part of ONE page that the call writes, for some kv heads and their query heads, so that a page's
+// maximum never leaves the workgroup.  D / 16 lanes hold a row: lane j the 8 elements from 8 j and their rotation partners
+// from D / 2 + 8 j, two 16-byte loads, no exchange for the rotation.  The row slots of a workgroup are split into
+// (token of the page) x (head): STEP (one row per sequence) gives them all to heads, otherwise tokens come first.  A lane
+// keeps its tokens while it walks the heads, so an angle is computed once per workgroup and not once per head: in fp64 as
+// turns (pos * theta^(-2i/D) / 2 pi, only the fraction kept), because an fp32 product at position 30000 is off by 1e-3.
+#include "paged.hip.h"
+
+#include <math.h>
+
+namespace cactus_hip {
+
+namespace {
+
+__device__ __forceinline__ float finite_half(float x) {
+    return x != x ? 0.0f : fminf(fmaxf(x, -65504.0f), 65504.0f);
+}
+
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, LPR);
+    return v;
+}
+template <int LPR>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, LPR));
+    return v;
+}
+
+struct Row16 {
+    float lo[8], hi[8];   // elements 8 j .. and D / 2 + 8 j ..
+};
+
+template <int D>
+__device__ __forceinline__ Row16 load_row(const uint16_t* __restrict__ row, int j) {
+    const v8h a = *reinterpret_cast<const v8h*>(row + 8 * j), b = *reinterpret_cast<const v8h*>(row + D / 2 + 8 * j);
+    Row16 r;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        r.lo[e] = (float)a[e];
+        r.hi[e] = (float)b[e];
+    }
+    return r;
+}
+
+// rms_norm with an optional weight, then the rotation by the angle whose cosine and sine the lane holds
+template <int D>
+__device__ __forceinline__ void norm_rotate(Row16& r, bool norm, const Row16& w, float eps, bool rotate, const float (&cs)[8],
+                                            const float (&sn)[8]) {
+    if (norm) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss = fmaf(r.hi[e], r.hi[e], fmaf(r.lo[e], r.lo[e], ss));
+        ss = row_sum<D / 16>(ss);
+        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            r.lo[e] = r.lo[e] * inv * w.lo[e];
+            r.hi[e] = r.hi[e] * inv * w.hi[e];
+        }
+    }
+    if (rotate) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float a = r.lo[e], b = r.hi[e];
+            r.lo[e] = a * cs[e] - b * sn[e];
+            r.hi[e] = b * cs[e] + a * sn[e];
+        }
+    }
+}
+
+__device__ __forceinline__ float absmax(const Row16& r) {
+    float m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) m = fmaxf(m, fmaxf(fabsf(r.lo[e]), fabsf(r.hi[e])));
+    return m;
+}
+
+template <int D>
+__device__ __forceinline__ void store_i8(int8_t* __restrict__ row, int j, const Row16& r, float inv) {
+    uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        o[e >> 2] |= (uint32_t)(clamp_i8(rne_i32(r.lo[e] * inv)) & 0xFF) << (8 * (e & 3));
+        o[2 + (e >> 2)] |= (uint32_t)(clamp_i8(rne_i32(r.hi[e] * inv)) & 0xFF) << (8 * (e & 3));
+    }
+    *reinterpret_cast<uint2*>(row + 8 * j) = make_uint2(o[0], o[1]);
+    *reinterpret_cast<uint2*>(row + D / 2 + 8 * j) = make_uint2(o[2], o[3]);
+}
+
+constexpr int MAX_SLOTS = 256;   // row slots of a workgroup (1024 threads, 4 lanes a row)
+
+template <int D, bool STEP>
+__global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArgs a) {
+    constexpr int LPR = D / 16;
+    constexpr int RPL = STEP ? 1 : 2;     // tokens a lane holds: the launch picks the workgroup so that 2 are enough
+    __shared__ uint32_t s_max[2][MAX_SLOTS];
+    __shared__ float s_again[2][MAX_SLOTS];      // old / new scale of a head whose earlier tokens are requantized, else 0
+
+    const int tid = threadIdx.x, slot = tid / LPR, j = tid % LPR, slots = blockDim.x / LPR;
+    const int P = 1 << a.c.page_shift;
+
+    // which sequence, which page of it, which of the page's slots
+    int b, seg = 0;
+    if constexpr (STEP) {
+        b = blockIdx.x;
+    } else {
+        const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, 1, P, 2); };
+        b = owner_of((int)blockIdx.x, a.batch, begin);
+        seg = (int)blockIdx.x - begin(b);
+    }
+    const Rows rows = rows_of(STEP ? nullptr : a.cu, b, a.tokens);
+    const long long pos0 = a.positions[b];
+    if (pos0 < 0 || seg < 0 || rows.count == 0) return;
+    const long long index = (pos0 >> a.c.page_shift) + seg, base = index << a.c.page_shift;   // page of the sequence, its first position
+    if (base >= pos0 + rows.count) return;
+    const int e_lo = (int)max(pos0 - base, 0LL), e_hi = (int)min(pos0 + rows.count - base, (long long)P);
+    const int row0 = rows.first + (int)(base - pos0);          // packed row of page slot 0
+    const int page = index < a.c.table_width ? page_of(a.c, b, (int)index) : -1;
+
+    const int TP = STEP ? 1 : min(P, slots), HP = slots / TP;  // tokens x heads of a pass
+    const int ts = slot % TP, hs = slot / TP;
+    float cs[RPL][8], sn[RPL][8];
+    int e[RPL];
+    bool live[RPL];
+#pragma unroll
+    for (int r = 0; r < RPL; r++) {
+        e[r] = STEP ? e_lo : ts + r * TP;
+        live[r] = e[r] >= e_lo && e[r] < e_hi;
+        if (a.rotate && live[r]) {
+            const double pos = (double)(base + e[r]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const double t = pos * a.rope.turn[8 * j + i];
+                sincospif(2.0f * (float)(t - floor(t)), &sn[r][i], &cs[r][i]);
+            }
+        }
+    }
+
+    const int kv0 = blockIdx.y * a.kv_per_group, kvn = min(a.kv_per_group, a.c.kv_heads - kv0);
+    Row16 kw{}, qw{};
+    if (a.k_weight) kw = load_row<D>(a.k_weight, j);
+    if (a.q_weight) qw = load_row<D>(a.q_weight, j);
+
+    if (page >= 0) {
+        for (int h0 = 0; h0 < kvn; h0 += HP) {
+            const int h = kv0 + h0 + hs;
+            const bool head = h0 + hs < kvn;
+            const size_t ph = (size_t)page * a.c.kv_heads + h;
+            float old_k = 0.0f, old_v = 0.0f;
+            if (head && e_lo > 0) {
+                old_k = a.c.ks[ph];
+                old_v = a.c.vs[ph];
+            }
+            if constexpr (!STEP) {
+                for (int i = tid; i < 2 * MAX_SLOTS; i += blockDim.x) (&s_max[0][0])[i] = 0;
+                __syncthreads();
+            }
+            Row16 kr[RPL], vr[RPL];
+            float mk = 0.0f, mv = 0.0f;
+#pragma unroll
+            for (int r = 0; r < RPL; r++) {
+                if (!head || !live[r]) continue;     // the same for all lanes of a row
+                const size_t row = (size_t)(row0 + e[r]);
+                kr[r] = load_row<D>(a.k + row * a.k_stride + (size_t)h * D, j);
+                vr[r] = load_row<D>(a.v + row * a.v_stride + (size_t)h * D, j);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    kr[r].lo[i] = finite_half(kr[r].lo[i]);
+                    kr[r].hi[i] = finite_half(kr[r].hi[i]);
+                    vr[r].lo[i] = finite_half(vr[r].lo[i]);
+                    vr[r].hi[i] = finite_half(vr[r].hi[i]);
+                }
+                norm_rotate<D>(kr[r], a.k_weight != nullptr, kw, a.eps, a.rotate, cs[r], sn[r]);
+                mk = fmaxf(mk, absmax(kr[r]));
+                mv = fmaxf(mv, absmax(vr[r]));
+            }
+            mk = row_max<LPR>(mk);
+            mv = row_max<LPR>(mv);
+            if constexpr (!STEP) {
+                if (j == 0 && head) {   // bits of non-negative floats order as the floats do: the maximum is the same in any order
+                    atomicMax(&s_max[0][hs], __float_as_uint(mk));
+                    atomicMax(&s_max[1][hs], __float_as_uint(mv));
+                }
+                __syncthreads();
+                mk = __uint_as_float(s_max[0][hs]);
+                mv = __uint_as_float(s_max[1][hs]);
+            }
+            const float new_k = fmaxf(old_k, fmaxf(mk / 127.0f, 1e-10f)), new_v = fmaxf(old_v, fmaxf(mv / 127.0f, 1e-10f));
+            const float inv_k = 1.0f / new_k, inv_v = 1.0f / new_v;
+#pragma unroll
+            for (int r = 0; r < RPL; r++) {
+                if (!head || !live[r]) continue;
+                const size_t at = (ph << a.c.page_shift) + e[r];
+                store_i8<D>(a.c.k + at * D, j, kr[r], inv_k);
+                store_i8<D>(a.c.v + at * D, j, vr[r], inv_v);
+            }
+            if (head && ts == 0 && j == 0) {
+                a.c.ks[ph] = new_k;
+                a.c.vs[ph] = new_v;
+                s_again[0][hs] = e_lo > 0 && new_k > old_k ? old_k / new_k : -1.0f;
+                s_again[1][hs] = e_lo > 0 && new_v > old_v ? old_v / new_v : -1.0f;
+            }
+            if (e_lo > 0) {             // the page held tokens before: bring them to a scale that has grown
+                __syncthreads();
+                for (int w = 0; w < 2 * min(HP, kvn - h0); w++) {
+                    const float f = s_again[w & 1][w >> 1];
+                    if (f < 0.0f) continue;
+                    const size_t first = (((size_t)page * a.c.kv_heads + kv0 + h0 + (w >> 1)) << a.c.page_shift) * D;
+                    int8_t* x = ((w & 1) ? a.c.v : a.c.k) + first;
+                    for (int i = tid * 16; i < e_lo * D; i += blockDim.x * 16) {
+                        v4i q = *reinterpret_cast<const v4i*>(x + i);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            uint32_t o = 0;
+#pragma unroll
+                            for (int s = 0; s < 4; s++)
+                                o |= (uint32_t)(rne_i32((float)(int8_t)((uint32_t)q[c] >> (8 * s)) * f) & 0xFF) << (8 * s);
+                            q[c] = (int)o;
+                        }
+                        *reinterpret_cast<v4i*>(x + i) = q;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+
+    if (a.q) {
+        const int g = a.q_heads / a.c.kv_heads, q0 = kv0 * g, qn = kvn * g;
+        for (int h0 = hs; h0 < qn; h0 += HP) {
+#pragma unroll
+            for (int r = 0; r < RPL; r++) {
+                if (!live[r]) continue;
+                const size_t row = (size_t)(row0 + e[r]);
+                Row16 x = load_row<D>(a.q + row * a.q_stride + (size_t)(q0 + h0) * D, j);
+                norm_rotate<D>(x, a.q_weight != nullptr, qw, a.eps, a.rotate, cs[r], sn[r]);
+                v8h lo, hi;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    lo[i] = (_Float16)x.lo[i];
+                    hi[i] = (_Float16)x.hi[i];
+                }
+                uint16_t* out = a.q_out + (row * a.q_heads + q0 + h0) * D;
+                *reinterpret_cast<v8h*>(out + 8 * j) = lo;
+                *reinterpret_cast<v8h*>(out + D / 2 + 8 * j) = hi;
+            }
+        }
+    }
+}
+
+// Read: a lane turns 16 bytes of a token into 32.  A wave walks the 16-byte pieces of its tokens in memory order; it looks up
+// the sequence of its first token and moves on from there.
+template <int D>
+__global__ __launch_bounds__(256) void read_paged_kernel(const PagedReadArgs a) {
+    const int chunks = a.c.kv_heads * (D / 16);              // 16-byte pieces of a token, keys or values
+    const long long total = (long long)a.rows * chunks;
+    const long long first = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+    if (first >= total) return;
+    int b = owner_of((int)(first / chunks), a.batch, [&](int i) { return min(max(a.cu[i], 0), a.rows); });
+    const long long at = first + (threadIdx.x & 63);
+    if (at >= total) return;
+    const int row = (int)(at / chunks), piece = (int)(at % chunks), h = piece / (D / 16), d = piece % (D / 16) * 16;
+    while (b < a.batch && row >= a.cu[b + 1]) b++;
+    if (b >= a.batch || row < a.cu[b]) return;
+    const long long token = (long long)a.starts[b] + (row - a.cu[b]);
+    const int page = token < 0 || (token >> a.c.page_shift) >= a.c.table_width ? -1 : page_of(a.c, b, (int)(token >> a.c.page_shift));
+    const size_t ph = (size_t)max(page, 0) * a.c.kv_heads + h;
+    const size_t src = ((ph << a.c.page_shift) + (size_t)(token & ((1 << a.c.page_shift) - 1))) * D + d;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        uint16_t* out = (which ? a.v_out : a.k_out) + ((size_t)row * a.c.kv_heads + h) * D + d;
+        v8h lo{}, hi{};
+        if (page >= 0) {
+            const float s = (which ? a.c.vs : a.c.ks)[ph];
+            const v4i q = *reinterpret_cast<const v4i*>((which ? a.c.v : a.c.k) + src);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                lo[e] = (_Float16)((float)(int8_t)((uint32_t)q[e >> 2] >> (8 * (e & 3))) * s);
+                hi[e] = (_Float16)((float)(int8_t)((uint32_t)q[2 + (e >> 2)] >> (8 * (e & 3))) * s);
+            }
+        }
+        *reinterpret_cast<v8h*>(out) = lo;
+        *reinterpret_cast<v8h*>(out + 8) = hi;
+    }
+}
+
+template <int D>
+hipError_t append_paged(const PagedAppendArgs& args, hipStream_t st) {
+    PagedAppendArgs a = args;
+    const int P = 1 << a.c.page_shift, LPR = D / 16;
+    const bool step = a.cu == nullptr;
+    // a workgroup per page piece and group of kv heads.  A step: 256 threads hold 256 / LPR heads at once.  Otherwise as
+    // many threads as let two tokens per lane cover a page.
+    const int threads = step ? 256 : (P * LPR / 2 < 256 ? 256 : P * LPR / 2);
+    const size_t pieces = step ? (size_t)a.batch : ((size_t)a.tokens >> a.c.page_shift) + 2 * (size_t)a.batch;
+    a.kv_per_group = a.c.kv_heads;
+    const dim3 grid((unsigned)pieces, (unsigned)((a.c.kv_heads + a.kv_per_group - 1) / a.kv_per_group));
+    if (step)
+        append_paged_kernel<D, true><<<grid, dim3(threads), 0, st>>>(a);
+    else
+        append_paged_kernel<D, false><<<grid, dim3(threads), 0, st>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_kv_append_paged(int head_dim, const PagedAppendArgs& a, hipStream_t st) {
+    return head_dim == 64 ? append_paged<64>(a, st) : head_dim == 128 ? append_paged<128>(a, st) : append_paged<256>(a, st);
+}
+
+hipError_t launch_kv_read_paged(int head_dim, const PagedReadArgs& a, hipStream_t st) {
+    const size_t pieces = (size_t)a.rows * a.c.kv_heads * (head_dim / 16);
+    const dim3 grid((unsigned)((pieces + 255) / 256));
+    if (head_dim == 64)
+        read_paged_kernel<64><<<grid, dim3(256), 0, st>>>(a);
+    else if (head_dim == 128)
+        read_paged_kernel<128><<<grid, dim3(256), 0, st>>>(a);
+    else
+        read_paged_kernel<256><<<grid, dim3(256), 0, st>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace cactus_hip

@@ -1,0 +1,67 @@
+// Internal launcher declarations of the paged cache (include/cactus_hip_paged.h).  Operands are checked by paged_api.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace cactus_hip {
+
+struct PagedCache {
+    int8_t* k;
+    int8_t* v;
+    float* ks;
+    float* vs;
+    const int32_t* tables;
+    int num_pages, table_width, page_shift, kv_heads;
+};
+
+// rotation frequencies of a head in turns per position: theta^(-2i / D) / (2 pi).  They travel as a kernel argument
+struct RopeTurns {
+    double turn[128];
+};
+
+struct PagedAppendArgs {
+    PagedCache c;
+    const int32_t* positions;
+    const int32_t* cu;         // null: one row per sequence
+    int batch, tokens;
+    const uint16_t *k, *v, *q;
+    size_t k_stride, v_stride, q_stride;
+    uint16_t* q_out;
+    int q_heads;
+    const uint16_t *q_weight, *k_weight;
+    float eps;
+    int rotate;
+    int kv_per_group;          // kv heads a workgroup takes
+    RopeTurns rope;
+};
+hipError_t launch_kv_append_paged(int head_dim, const PagedAppendArgs& a, hipStream_t st);
+
+struct PagedReadArgs {
+    PagedCache c;
+    const int32_t* starts;
+    const int32_t* cu;
+    int batch, rows;
+    uint16_t *k_out, *v_out;
+};
+hipError_t launch_kv_read_paged(int head_dim, const PagedReadArgs& a, hipStream_t st);
+
+struct PagedAttnArgs {
+    PagedCache c;              // paged attention
+    const int32_t* contexts;
+    const uint16_t *k, *v;     // ragged attention
+    size_t k_stride, v_stride;
+    const int32_t* cu;         // null: one row per sequence
+    int batch, tokens;
+    const uint16_t* q;
+    size_t q_stride;
+    uint16_t* out;
+    int q_heads, kv_heads;
+    float scale;
+    int window, sink;
+};
+hipError_t launch_attention_paged(int head_dim, const PagedAttnArgs& a, hipStream_t st);
+hipError_t launch_attention_ragged(int head_dim, const PagedAttnArgs& a, hipStream_t st);
+
+}  // namespace cactus_hip

@@ -1,0 +1,53 @@
+// Device helpers shared by the kernels of the paged cache: packed rows, their owners, pages.
+#pragma once
+
+#include "common.hip.h"
+#include "paged.h"
+
+namespace cactus_hip {
+
+struct Rows {
+    int first, count;
+};
+
+// Rows of sequence b.  cu is device data that nobody checked: whatever it holds, the rows stay inside [0, tokens).
+__device__ __forceinline__ Rows rows_of(const int32_t* __restrict__ cu, int b, int tokens) {
+    if (!cu) return Rows{b, 1};
+    const int lo = min(max(cu[b], 0), tokens), hi = min(max(cu[b + 1], lo), tokens);
+    return Rows{lo, hi - lo};
+}
+
+// The last b in [0, batch) with begin(b) <= w, for begin not decreasing and begin(0) <= w: 64 candidates at a time, one per
+// lane, so 256 sequences take two dependent loads instead of eight.  All 64 lanes of the wave call it.
+template <class Begin>
+__device__ __forceinline__ int owner_of(int w, int batch, Begin begin) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = batch;
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const int at = lane * step;
+        const bool reached = at < n && begin(lo + at) <= w;
+        const int c = max(__popcll(__ballot(reached)), 1) - 1;
+        lo += c * step;
+        n = min(step, n - c * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Work of a ragged batch without its lengths on the host: sequence b owns the work slots floor(cu[b] * per / size) + extra * b
+// up to the next sequence's first one.  That is at least floor(rows * per / size) + extra slots for its rows * per items: with
+// extra 1 enough for pieces of `size` items that start at the sequence's first item (ceil), with extra 2 for pieces cut at
+// multiples of `size` of some other origin.  The launch takes floor(tokens * per / size) + extra * batch slots.
+__device__ __forceinline__ int slot_begin(const int32_t* __restrict__ cu, int b, int tokens, int per, int size, int extra) {
+    const int at = cu ? min(max(cu[b], 0), tokens) : b;
+    return (int)((long long)at * per / size) + extra * b;
+}
+
+// Page of tokens page_size * i .. of sequence b, or -1.
+__device__ __forceinline__ int page_of(const PagedCache& c, int b, int i) {
+    if (i < 0 || i >= c.table_width) return -1;
+    const int p = c.tables[(size_t)b * c.table_width + i];
+    return p >= 0 && p < c.num_pages ? p : -1;
+}
+
+}  // namespace cactus_hip
