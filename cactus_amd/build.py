@@ -29,7 +29,8 @@ FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # one-wave-per-tile kernel 126 instead of 168 + 32, and the copies out of the AGPRs go.
 EXTRA_FLAGS = {"matmul_gemm.hip": ["-fno-slp-vectorize"],
                "attention_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-               "matmul_skinny.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+               "matmul_skinny.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "attention_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _stale(target, deps):

@@ -60,8 +60,16 @@ struct PagedAttnArgs {
     int q_heads, kv_heads;
     float scale;
     int window, sink;
+    float* work;               // split records: per (item, split) work_rows x (maximum, sum) and work_rows x [head_dim]
+    int work_rows;
 };
-hipError_t launch_attention_paged(int head_dim, const PagedAttnArgs& a, hipStream_t st);
+// how a call with few rows per sequence is cut: row tiles per (sequence, kv head), rows kept per record, key splits
+struct StepShape {
+    int row_tiles, rows, splits;
+};
+StepShape step_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
+                     bool one_row_each);
+hipError_t launch_attention_paged(int head_dim, const PagedAttnArgs& a, const StepShape& s, hipStream_t st);
 hipError_t launch_attention_ragged(int head_dim, const PagedAttnArgs& a, hipStream_t st);
 
 }  // namespace cactus_hip

@@ -172,7 +172,9 @@ int cactus_hip_kv_read_paged_f16_dev(const cactus_hip_paged_kv* cache, const int
 size_t cactus_hip_attention_paged_workspace_bytes(const cactus_hip_paged_kv* cache, size_t batch, size_t tokens,
                                                   size_t max_context, size_t num_q_heads, size_t window, size_t sink,
                                                   int one_row_each) {
-    return 0;
+    if (!cache || batch == 0 || tokens == 0 || bad_groups(num_q_heads, cache->kv_heads) || batch > MAX_BATCH) return 0;
+    const StepShape s = step_shape(batch, tokens, max_context, num_q_heads, cache->kv_heads, window, sink, one_row_each != 0);
+    return s.splits == 1 ? 0 : batch * cache->kv_heads * s.row_tiles * s.splits * s.rows * (cache->head_dim + 2) * sizeof(float);
 }
 
 int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const int32_t* block_tables, size_t table_width,
@@ -204,7 +206,14 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
     a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)cache->head_dim) : scale;
     a.window = (int)window;
     a.sink = (int)sink;
-    return launched(who, launch_attention_paged((int)cache->head_dim, a, (hipStream_t)stream));
+    const size_t need = cactus_hip_attention_paged_workspace_bytes(cache, batch, tokens, max_context, num_q_heads, window, sink,
+                                                                   cu_seqlens == nullptr);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return refuse(who, "workspace missing, too small or not 16-byte aligned");
+    const StepShape s = step_shape(batch, tokens, max_context, num_q_heads, cache->kv_heads, window, sink, cu_seqlens == nullptr);
+    a.work = static_cast<float*>(workspace);
+    a.work_rows = s.rows;
+    return launched(who, launch_attention_paged((int)cache->head_dim, a, s, (hipStream_t)stream));
 }
 
 int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride, const cactus_half_t* k, size_t k_stride,
