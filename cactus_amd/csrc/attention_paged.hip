@@ -99,20 +99,6 @@ struct StepBlock {
     int key;          // first key
 };
 
-// Rows a wave works on and the blocks of keys they see: `sinks` blocks from 0, then [first, ..)
-struct StepPlan {
-    int sinks, first, blocks;
-};
-__device__ __forceinline__ StepPlan plan_blocks(long long pos_first, long long pos_last, int window, int sink, int size) {
-    StepPlan p;
-    const int all = pos_last < 0 ? 0 : (int)(pos_last / size) + 1;
-    const long long low = window ? pos_first - window : 0;
-    p.first = low > 0 ? (int)(low / size) : 0;
-    p.sinks = min(p.first, sink > 0 && window ? (int)(((long long)sink + size - 1) / size) : 0);
-    p.blocks = p.sinks + max(all - p.first, 0);
-    return p;
-}
-
 template <int D>
 __global__ __launch_bounds__(64 * STEP_WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : D == 128 ? 3 : 2)))
 void attention_step_kernel(const PagedAttnArgs a, const int splits, const int row_tiles) {
@@ -128,16 +114,16 @@ void attention_step_kernel(const PagedAttnArgs a, const int splits, const int ro
     const int R = min(rows.count * group - tile * STEP_ROWS, STEP_ROWS);       // rows of this tile
     // a ragged batch: sequences with more rows are the chunk kernel's
     if (R <= 0 || (a.cu && rows.count * group > STEP_ROWS)) return;
-    const long long context = min((long long)a.contexts[b], (long long)a.c.table_width << a.c.page_shift);
+    const int context = min(a.contexts[b], a.c.table_width << a.c.page_shift);
     const int row = tile * STEP_ROWS + min(n, R - 1);                          // lanes past the last row repeat it
     const int token = rows.first + row / group, qh = head * group + row % group;
-    const long long pos = context - rows.count + row / group;
-    const long long pos_first = context - rows.count + tile * STEP_ROWS / group;
-    const long long pos_last = context - rows.count + (tile * STEP_ROWS + R - 1) / group;
-    const StepPlan plan = plan_blocks(pos_first, pos_last, a.window, a.sink, STEP_KEYS);
+    const int pos = context - rows.count + row / group;
+    const int pos_first = context - rows.count + tile * STEP_ROWS / group;
+    const int pos_last = context - rows.count + (tile * STEP_ROWS + R - 1) / group;
+    const TilePlan plan = plan_tiles(pos_first, pos_last, a.window, a.sink, STEP_KEYS);
     // this workgroup's blocks: whole rounds of its waves, so that a short sequence uses few splits
-    const int rounds = (plan.blocks + STEP_WAVES - 1) / STEP_WAVES, per = (rounds + splits - 1) / splits * STEP_WAVES;
-    const int u0 = split * per + wave, u1 = min(split * per + per, plan.blocks);
+    const int rounds = (plan.tiles + STEP_WAVES - 1) / STEP_WAVES, per = (rounds + splits - 1) / splits * STEP_WAVES;
+    const int u0 = split * per + wave, u1 = min(split * per + per, plan.tiles);
 
     // Q^T: step 2 i + c contracts bytes 64 i + 16 g + 8 c .. of a key row
     v8h q[2 * KP];
@@ -393,96 +379,11 @@ hipError_t launch_step(const PagedAttnArgs& a, const StepShape& s, hipStream_t s
     return hipGetLastError();
 }
 
-template <int D, bool PAGED>
-__global__ __launch_bounds__(256) void attention_rows_kernel(const PagedAttnArgs a) {
-    __shared__ float s_q[4][D];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long long item = (long long)blockIdx.x * 4 + w;
-    if (item >= (long long)a.tokens * a.q_heads) return;
-    const int row = (int)(item / a.q_heads), h = (int)(item % a.q_heads), kvh = h / (a.q_heads / a.kv_heads);
-    const int b = a.cu ? owner_of(row, a.batch, [&](int i) { return min(max(a.cu[i], 0), a.tokens); }) : row;
-    const Rows rows = rows_of(a.cu, b, a.tokens);
-    if (row < rows.first || row >= rows.first + rows.count) return;
-    long long context = rows.count;
-    if (PAGED) context = min((long long)a.contexts[b], (long long)a.c.table_width << a.c.page_shift);
-    const long long pos = context - rows.count + (row - rows.first);
-    const uint16_t* qr = a.q + (size_t)row * a.q_stride + (size_t)h * D;
-    for (int d = lane; d < D; d += 64) s_q[w][d] = h2f(qr[d]);
-    __builtin_amdgcn_wave_barrier();
-
-    constexpr int DPL = D / 64;
-    float o[DPL], m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < DPL; i++) o[i] = 0.0f;
-    const long long low = a.window ? max(0LL, pos - a.window) : 0;
-    for (long long k0 = 0; k0 <= pos; k0 += 64) {
-        if (k0 + 64 <= low && k0 >= a.sink) {      // nothing here is seen
-            continue;
-        }
-        const long long key = k0 + lane;
-        bool seen = key <= pos && (!a.window || pos - key <= a.window || key < a.sink);
-        int page = -1;
-        size_t ph = 0;
-        if (PAGED) {
-            if (seen) page = page_of(a.c, b, (int)(key >> a.c.page_shift));
-            seen = seen && page >= 0;
-            ph = (size_t)max(page, 0) * a.kv_heads + kvh;
-        }
-        float s = -INFINITY, vscale = 1.0f;
-        if (seen) {
-            s = 0.0f;
-            if (PAGED) {
-                const int8_t* kr = a.c.k + ((ph << a.c.page_shift) + (key & ((1 << a.c.page_shift) - 1))) * D;
-                for (int d = 0; d < D; d++) s = fmaf(s_q[w][d], (float)kr[d], s);
-                s *= a.c.ks[ph];
-                vscale = a.c.vs[ph];
-            } else {
-                const uint16_t* kr = a.k + (size_t)(rows.first + key) * a.k_stride + (size_t)kvh * D;
-                for (int d = 0; d < D; d++) s = fmaf(s_q[w][d], h2f(kr[d]), s);
-            }
-            s *= a.scale;
-        }
-        const float mn = fmaxf(m, wave_max(s));
-        if (mn == -INFINITY) continue;
-        const float p = seen ? __expf(s - mn) : 0.0f, f = __expf(m - mn);
-        m = mn;
-        l = l * f + wave_sum(p);
-        for (int i = 0; i < DPL; i++) o[i] *= f;
-        for (int t = 0; t < 64; t++) {
-            const float pt = __shfl(p, t);
-            if (pt == 0.0f) continue;
-            if (PAGED) {
-                const size_t ph_t = (size_t)__shfl(page, t) * a.kv_heads + kvh;
-                const float pv = pt * __shfl(vscale, t);
-                const int8_t* vr = a.c.v + ((ph_t << a.c.page_shift) + ((k0 + t) & ((1 << a.c.page_shift) - 1))) * D;
-                for (int i = 0; i < DPL; i++) o[i] = fmaf(pv, (float)vr[lane + 64 * i], o[i]);
-            } else {
-                const uint16_t* vr = a.v + (size_t)(rows.first + k0 + t) * a.v_stride + (size_t)kvh * D;
-                for (int i = 0; i < DPL; i++) o[i] = fmaf(pt, h2f(vr[lane + 64 * i]), o[i]);
-            }
-        }
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    uint16_t* out = a.out + ((size_t)row * a.q_heads + h) * D;
-    for (int i = 0; i < DPL; i++) out[lane + 64 * i] = f2h(o[i] * inv);
-}
-
-template <bool PAGED>
-hipError_t launch_rows(int D, const PagedAttnArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)(((size_t)a.tokens * a.q_heads + 3) / 4));
-    if (D == 64)
-        attention_rows_kernel<64, PAGED><<<grid, dim3(256), 0, st>>>(a);
-    else if (D == 128)
-        attention_rows_kernel<128, PAGED><<<grid, dim3(256), 0, st>>>(a);
-    else
-        attention_rows_kernel<256, PAGED><<<grid, dim3(256), 0, st>>>(a);
-    return hipGetLastError();
-}
-
 }  // namespace
 
 // The split rule.  A workgroup takes at least one block per wave (128 keys), and a batch is split until about 1024 workgroups
 // (four per CU) are there or nothing is left to split.
-StepShape step_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
+StepShape step_shape(size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
                      bool one_row_each) {
     StepShape s;
     const size_t group = q_heads / kv_heads;
@@ -497,10 +398,8 @@ StepShape step_shape(size_t batch, size_t tokens, size_t max_context, size_t q_h
     return s;
 }
 
-hipError_t launch_attention_paged(int D, const PagedAttnArgs& a, const StepShape& s, hipStream_t st) {
-    if (a.cu) return launch_rows<true>(D, a, st);
+hipError_t launch_attention_step(int D, const PagedAttnArgs& a, const StepShape& s, hipStream_t st) {
     return D == 64 ? launch_step<64>(a, s, st) : D == 128 ? launch_step<128>(a, s, st) : launch_step<256>(a, s, st);
 }
-hipError_t launch_attention_ragged(int D, const PagedAttnArgs& a, hipStream_t st) { return launch_rows<false>(D, a, st); }
 
 }  // namespace cactus_hip

@@ -1,0 +1,445 @@
+// Attention of many query rows (include/cactus_hip_paged.h): packed FP16 prompts, and prompt chunks over the paged INT8
+// cache.  Bound: matrix cores and the softmax's vector instructions, which share a SIMD's issue port.
+//
+// A workgroup is four waves on 128 consecutive rows of one (sequence, kv head); a row is (token, query head of the group), so a
+// key tile in LDS serves all query heads of its kv head.  A wave owns 32 rows and computes everything transposed, a lane
+// owning a row (lane % 32):
+//   S^T = K Q^T   v_mfma_f32_32x32x16_f16, K rows from LDS, the wave's Q in registers for the whole kernel
+//   O^T = V^T P^T V^T through the transposing LDS read (ds_read_b64_tr_b16); P is the lane's own scores, in the key order the
+//                 first product left them in (the contraction order is free)
+// so the softmax's maximum and sum are in-lane work plus one exchange with lane ^ 32, and weights never move.  The rest is the
+// online softmax in base 2; (l, O) move to a new maximum only when it has grown by more than 2^8.
+// Key tiles (64 keys, 32 at head_dim 256) are double-buffered: the next one is loaded into registers before the current one is
+// computed and stored to the other buffer behind it, one barrier per tile.  16-byte chunks of a row are swizzled so that neither
+// the row reads of K (16 rows, one chunk) nor the transposed reads of V (4 rows, 4 chunks) meet on a bank.
+// INT8 pages become halves on the way into LDS: keys as the subnormal (b + 128) 2^-24 (one v_perm per two; the offset leaves
+// with the score's fma), values as b 2^-9.  Page scales enter as in attention_paged.hip.
+// Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count); everything else is fp32.
+#include "paged.hip.h"
+
+#include <math.h>
+
+#include <type_traits>
+
+namespace cactus_hip {
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int TILE_ROWS = 128;
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef unsigned short v8u __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+
+__device__ __forceinline__ float pair_max(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 16-byte chunk at which chunk c of a row lies in LDS
+template <int D>
+__device__ __forceinline__ int k_chunk(int row, int c) { return D == 64 ? c ^ ((row >> 1) & 7) : c ^ (row & 15); }
+template <int D>
+__device__ __forceinline__ int v_chunk(int row, int c) { return D == 64 ? c ^ ((row & 2) << 1) : c ^ ((row & 3) << 2); }
+
+// four bytes, each ^ 0x80, as halves (b + 128) 2^-24
+__device__ __forceinline__ void offset_halves(uint32_t x, uint32_t& lo, uint32_t& hi) {
+    lo = __builtin_amdgcn_perm(0u, x, 0x0c010c00u);
+    hi = __builtin_amdgcn_perm(0u, x, 0x0c030c02u);
+}
+// (b + 128) 2^-24 -> b 2^-9
+__device__ __forceinline__ uint32_t centred(uint32_t u) {
+    const _Float16 up = (_Float16)32768.0f, down = (_Float16)-0.25f;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, u), v2h{up, up}, v2h{down, down}));
+}
+
+// One key tile on its way from memory to LDS: 16-byte pieces, and (paged) the scales of its 16-key groups
+template <int D, bool PAGED>
+struct TileLoad {
+    static constexpr int BK = D == 256 ? 32 : 64;
+    static constexpr int PIECES = BK * D * (PAGED ? 1 : 2) / 16 / 256;      // per thread and operand
+    v4i k[PIECES], v[PIECES];
+    float scale;         // lane 2 g + (0 key, 1 value) of the first wave: the scale of 16-key group g
+};
+
+template <int D, bool PAGED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int slots) {
+    using Load = TileLoad<D, PAGED>;
+    constexpr int BK = Load::BK, KT = BK / 32, GROUPS = BK / 16, NST = D / 16, NDT = D / 32, ROW = D * 2;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_k[2][BK * ROW];
+    __shared__ __attribute__((aligned(1024))) unsigned char s_v[2][BK * ROW];
+    __shared__ float s_scale[2][GROUPS][2];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    // kv heads go round first (a head's rows stay in one XCD's L2 when their number divides by 8), heavy slots early
+    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads;
+    const int group = a.q_heads / a.kv_heads;
+    const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
+    const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
+    const Rows rows = rows_of(a.cu, b, a.tokens);
+    const int R = tile < 0 ? 0 : min(rows.count * group - tile * TILE_ROWS, TILE_ROWS);
+    if (R <= 0 || (PAGED && rows.count * group <= a.min_rows)) return;
+    int context = rows.count;
+    if (PAGED) context = min(a.contexts[b], a.c.table_width << a.c.page_shift);
+    const int pos0 = context - rows.count;                    // position of the sequence's first row
+    const auto pos_of = [&](int r) { return pos0 + (tile * TILE_ROWS + r) / group; };
+    const int row = min(wave * 32 + n, R - 1);                       // lanes past the last row repeat it
+    const int orow = tile * TILE_ROWS + row, token = rows.first + orow / group, qh = head * group + orow % group;
+    const int pos = pos0 + orow / group;
+    const int wpos_first = pos_of(min(wave * 32, R - 1)), wpos_last = pos_of(min(wave * 32 + 31, R - 1));
+    const int last = pos_of(R - 1);
+    const TilePlan plan = plan_tiles(pos_of(0), last, a.window, a.sink, BK);
+    const int per = (plan.tiles + splits - 1) / splits, u0 = split * per, u1 = min(u0 + per, plan.tiles);
+
+    // Q^T; a negative scale is moved into Q, so that the largest score is the largest product
+    v8h q[NST];
+    float bias = 0.0f;
+    {
+        const uint16_t* qr = a.q + (size_t)token * a.q_stride + (size_t)qh * D;
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int s = 0; s < NST; s++) {
+            v4i x = *reinterpret_cast<const v4i*>(qr + 16 * s + 8 * h);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] ^= (int)flip;
+            q[s] = __builtin_bit_cast(v8h, x);
+            if (PAGED)
+#pragma unroll
+                for (int e = 0; e < 8; e++) bias += (float)q[s][e];
+        }
+        if (PAGED) bias = pair_sum(bias) * -128.0f;
+    }
+    const float c0 = fabsf(a.scale) * LOG2E;
+
+    const auto key_of = [&](int u) { return (u < plan.sinks ? u : u - plan.sinks + plan.first) * BK; };
+    // page of the 16 keys from `key0`, or -1
+    const auto page_at = [&](int key0) { return key0 <= last ? page_of(a.c, b, key0 >> a.c.page_shift) : -1; };
+    int pages[Load::PIECES], my_page = -1;                           // of the tile after the next
+    const auto look_up = [&](int u) {
+        if constexpr (PAGED) {
+            if (u >= u1) return;
+            const int key = key_of(u);
+#pragma unroll
+            for (int i = 0; i < Load::PIECES; i++) {
+                const int r = (i * 256 + wave * 64) / (D / 16);      // the wave's rows lie in one 16-key group
+                pages[i] = page_at(key + (r & ~15));
+            }
+            if (tid < 2 * GROUPS) my_page = page_at(key + 16 * (tid >> 1));
+        }
+    };
+    const auto fetch = [&](Load& t, int u) {
+        const int key = key_of(u);
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < Load::PIECES; i++) {
+                const int p = i * 256 + tid, r = p / (D / 16), d = p % (D / 16) * 16, page = __builtin_amdgcn_readfirstlane(pages[i]);
+                const int at = (key + r) & ((1 << a.c.page_shift) - 1);
+                const size_t from = ((((size_t)max(page, 0) * a.kv_heads + head) << a.c.page_shift) + at) * D + d;
+                t.k[i] = *reinterpret_cast<const v4i*>(a.c.k + from);
+                t.v[i] = *reinterpret_cast<const v4i*>(a.c.v + from);
+            }
+            if (tid < 2 * GROUPS)
+                t.scale = my_page < 0 ? -1.0f : fmaxf((tid & 1 ? a.c.vs : a.c.ks)[(size_t)my_page * a.kv_heads + head], 0.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Load::PIECES; i++) {
+                const int p = i * 256 + tid, r = p / (D / 8), d = p % (D / 8) * 8;
+                const size_t from = (size_t)(rows.first + min(key + r, last));   // past the last key: that key again
+                t.k[i] = *reinterpret_cast<const v4i*>(a.k + from * a.k_stride + (size_t)head * D + d);
+                t.v[i] = *reinterpret_cast<const v4i*>(a.v + from * a.v_stride + (size_t)head * D + d);
+            }
+        }
+    };
+    const auto stash = [&](const Load& t, int buf) {
+#pragma unroll
+        for (int i = 0; i < Load::PIECES; i++) {
+            const int p = i * 256 + tid;
+            if constexpr (PAGED) {
+                const int r = p / (D / 16), c = p % (D / 16) * 2;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    v4i x, y;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        uint32_t lo, hi;
+                        offset_halves((uint32_t)t.k[i][2 * w + e] ^ 0x80808080u, lo, hi);
+                        x[2 * e] = (int)lo;
+                        x[2 * e + 1] = (int)hi;
+                        offset_halves((uint32_t)t.v[i][2 * w + e] ^ 0x80808080u, lo, hi);
+                        y[2 * e] = (int)centred(lo);
+                        y[2 * e + 1] = (int)centred(hi);
+                    }
+                    *reinterpret_cast<v4i*>(s_k[buf] + r * ROW + k_chunk<D>(r, c + w) * 16) = x;
+                    *reinterpret_cast<v4i*>(s_v[buf] + r * ROW + v_chunk<D>(r, c + w) * 16) = y;
+                }
+            } else {
+                const int r = p / (D / 8), c = p % (D / 8);
+                *reinterpret_cast<v4i*>(s_k[buf] + r * ROW + k_chunk<D>(r, c) * 16) = t.k[i];
+                *reinterpret_cast<v4i*>(s_v[buf] + r * ROW + v_chunk<D>(r, c) * 16) = t.v[i];
+            }
+        }
+        if (PAGED && tid < 2 * GROUPS) s_scale[buf][tid >> 1][tid & 1] = t.scale;
+    };
+
+    float m = -1e30f, l = 0.0f;
+    v16f o[NDT];
+#pragma unroll
+    for (int i = 0; i < NDT; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[i][r] = 0.0f;
+
+    // lane addresses: K row n of a 32-key half, chunk 2 s + h; V key 4 h + tq, dims 16 (gi & 1) + 4 tp .. of a 32-dim tile
+    const int tq = (lane >> 2) & 3, tp = lane & 3, gi = (lane >> 4) & 1;
+    const auto compute = [&](auto whole_tag, int u, int buf) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole_tag)::value;
+        const int key = key_of(u);
+        v16f s[KT];
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < NST; st++) {
+                const v8h kf = *reinterpret_cast<const v8h*>(s_k[buf] + (32 * t + n) * ROW + k_chunk<D>(n, 2 * st + h) * 16);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[st], s[t], 0, 0, 0);
+            }
+        }
+        float inv_vs[GROUPS];
+        bool live[GROUPS];
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                const float ks = s_scale[buf][g][0], v0 = s_scale[buf][g][1], vs = fmaxf(v0, 1e-20f);
+                live[g] = v0 >= 0.0f;
+                const float c = c0 * ks, up = c * 16777216.0f, add = fmaf(c, bias, __log2f(vs));
+                inv_vs[g] = 1.0f / vs;
+#pragma unroll
+                for (int r = 0; r < 8; r++) s[g >> 1][8 * (g & 1) + r] = fmaf(s[g >> 1][8 * (g & 1) + r], up, add);
+            }
+        }
+        if constexpr (!WHOLE) {
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int j = key + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
+                    bool seen = j <= pos && (!a.window || pos - j <= a.window || j < a.sink);
+                    if constexpr (PAGED) seen = seen && live[2 * t + (r >> 3)];
+                    s[t][r] = seen ? s[t][r] : -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(s[t][r], s[t][r + 1]), top);
+        top = pair_max(top);
+        if (!PAGED) top *= c0;
+        if (__any(top > m + 8.0f)) {
+            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < NDT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[i][r] *= f;
+        }
+        v8h p[2 * KT];
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            float w[8], sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const float x = s[g >> 1][8 * (g & 1) + r];
+                w[r] = __builtin_amdgcn_exp2f(PAGED ? x - m : fmaf(x, c0, -m));
+                sum += w[r];
+            }
+            l = PAGED ? fmaf(sum, inv_vs[g], l) : l + sum;
+#pragma unroll
+            for (int r = 0; r < 8; r += 2) {
+                const v2h two = __builtin_convertvector(v2f{w[r], w[r + 1]}, v2h);
+                p[g][r] = two[0];
+                p[g][r + 1] = two[1];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NDT; i++)
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                const int r = 16 * g + 4 * h + tq;
+                const unsigned char* at = s_v[buf] + r * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
+                const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
+                const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * ROW));
+                v8h vf = __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+                if constexpr (!PAGED && !WHOLE) {
+                    // a value that is not finite must not reach a row that does not see its key: 0 * inf is NaN
+                    const v4i x = __builtin_bit_cast(v4i, vf);
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) odd |= (((uint32_t)x[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                    if (__any(odd != 0)) {
+                        // the weights of +inf, -inf and NaN values of a dim are summed apart: any weight there is the result
+                        v8u y = __builtin_bit_cast(v8u, vf), mark;
+#pragma unroll 1
+                        for (int kind = 0; kind < 3; kind++) {
+                            const uint16_t lo = kind == 0 ? 0x7c00u : kind == 1 ? 0xfc00u : 0x7c01u;
+#pragma unroll
+                            for (int e = 0; e < 8; e++)
+                                mark[e] = (kind < 2 ? y[e] == lo : (y[e] & 0x7fffu) >= lo) ? 0x3c00u : 0u;     // 1 or 0
+                            v16f sum;
+#pragma unroll
+                            for (int r2 = 0; r2 < 16; r2++) sum[r2] = 0.0f;
+                            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, mark), p[g], sum, 0, 0, 0);
+                            const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+#pragma unroll
+                            for (int r2 = 0; r2 < 16; r2++) o[i][r2] += sum[r2] > 0.0f ? add : 0.0f;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; e++) y[e] = (y[e] & 0x7c00u) == 0x7c00u ? 0 : y[e];
+                        vf = __builtin_bit_cast(v8h, y);
+                    }
+                }
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[g], o[i], 0, 0, 0);
+            }
+    };
+
+    if (u0 < u1) {
+        Load t;
+        look_up(u0);
+        fetch(t, u0);
+        look_up(u0 + 1);
+        stash(t, 0);
+        __syncthreads();
+        for (int u = u0, buf = 0; u < u1; u++, buf ^= 1) {
+            if (u + 1 < u1) {
+                fetch(t, u + 1);
+                look_up(u + 2);
+            }
+            const int key = key_of(u);
+            if (key <= wpos_last && (!a.window || key + BK - 1 >= wpos_first - a.window || key < a.sink)) {
+                bool whole = key + BK - 1 <= wpos_first && (!a.window || key >= wpos_last - a.window || key + BK - 1 < a.sink);
+                if constexpr (PAGED) {
+#pragma unroll
+                    for (int g = 0; g < GROUPS; g++) whole = whole && s_scale[buf][g][1] >= 0.0f;
+                    whole = __builtin_amdgcn_readfirstlane(whole);
+                }
+                if (whole)
+                    compute(std::true_type{}, u, buf);
+                else
+                    compute(std::false_type{}, u, buf);
+            }
+            if (u + 1 < u1) stash(t, buf ^ 1);
+            __syncthreads();
+        }
+    }
+
+    l = pair_sum(l);
+    if (wave * 32 + n >= R) return;
+    const float unit = PAGED ? 512.0f : 1.0f;
+    if (splits > 1) {
+        float* record = a.work + (size_t)blockIdx.x * TILE_ROWS * (D + 2);
+        if (h == 0) {
+            record[2 * row] = m;
+            record[2 * row + 1] = l;
+        }
+        float* out = record + 2 * TILE_ROWS + (size_t)row * D;
+#pragma unroll
+        for (int i = 0; i < NDT; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                v4f x;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = o[i][r + e] * unit;
+                *reinterpret_cast<v4f*>(out + 32 * i + 2 * r + 4 * h) = x;
+            }
+    } else {
+        const float inv = l > 0.0f || l != l ? unit / l : 0.0f;
+        uint16_t* out = a.out + ((size_t)token * a.q_heads + qh) * D;
+#pragma unroll
+        for (int i = 0; i < NDT; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                v4h x;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = (_Float16)(o[i][r + e] * inv);
+                *reinterpret_cast<v4h*>(out + 32 * i + 2 * r + 4 * h) = x;
+            }
+    }
+}
+
+// joins the splits of a tile's rows: a wave per row, lanes = dims
+template <int D>
+__global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int splits, const int slots) {
+    const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = blockIdx.x, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads, group = a.q_heads / a.kv_heads;
+    const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
+    const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
+    const Rows rows = rows_of(a.cu, b, a.tokens);
+    const int orow = tile * TILE_ROWS + row;
+    if (tile < 0 || orow >= rows.count * group || rows.count * group <= a.min_rows) return;
+    constexpr size_t step = (size_t)TILE_ROWS * (D + 2);
+    const float* rec = a.work + (size_t)id * splits * step;
+    float m = -1e30f, l = 0.0f;
+    for (int s = 0; s < splits; s++) m = fmaxf(m, rec[s * step + 2 * row]);
+    constexpr int W = D / 64;
+    float o[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) o[i] = 0.0f;
+    for (int s = 0; s < splits; s++) {
+        const float f = __builtin_amdgcn_exp2f(rec[s * step + 2 * row] - m);
+        l = fmaf(rec[s * step + 2 * row + 1], f, l);
+        const float* x = rec + s * step + 2 * TILE_ROWS + (size_t)row * D + lane * W;
+#pragma unroll
+        for (int i = 0; i < W; i++) o[i] = fmaf(x[i], f, o[i]);
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    uint16_t* out = a.out + ((size_t)(rows.first + orow / group) * a.q_heads + head * group + orow % group) * D + lane * W;
+#pragma unroll
+    for (int i = 0; i < W; i++) out[i] = f2h(o[i] * inv);
+}
+
+template <int D, bool PAGED>
+hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
+    const size_t items = (size_t)s.slots * a.kv_heads;
+    attention_tile_kernel<D, PAGED><<<dim3((unsigned)(items * s.splits)), dim3(256), 0, st>>>(a, s.splits, s.slots);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || s.splits == 1) return e;
+    attention_tile_join_kernel<D><<<dim3((unsigned)items, TILE_ROWS / 4), dim3(256), 0, st>>>(a, s.splits, s.slots);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// A tile kernel's launch: a slot per 128 rows of a sequence and kv head, and key splits where that leaves most of the chip idle:
+// as many as fill it twice over, each with at least 512 keys.
+TileShape tile_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink) {
+    TileShape s;
+    s.slots = (int)(tokens * (q_heads / kv_heads) / TILE_ROWS + batch);
+    const size_t items = (size_t)s.slots * kv_heads;
+    size_t keys = max_context;
+    if (window && window + sink + TILE_ROWS < keys) keys = window + sink + TILE_ROWS;
+    const size_t most = keys / 512, want = 512 / items;
+    s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
+    return s;
+}
+size_t tile_record_floats(size_t head_dim) { return TILE_ROWS * (head_dim + 2); }
+
+hipError_t launch_attention_tiles(int D, bool paged, const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
+    if (paged) return D == 64 ? launch<64, true>(a, s, st) : D == 128 ? launch<128, true>(a, s, st) : launch<256, true>(a, s, st);
+    return D == 64 ? launch<64, false>(a, s, st) : D == 128 ? launch<128, false>(a, s, st) : launch<256, false>(a, s, st);
+}
+
+}  // namespace cactus_hip

@@ -62,14 +62,22 @@ struct PagedAttnArgs {
     int window, sink;
     float* work;               // split records: per (item, split) work_rows x (maximum, sum) and work_rows x [head_dim]
     int work_rows;
+    int min_rows;              // tile kernel: sequences with at most that many rows per kv head are not its
 };
-// how a call with few rows per sequence is cut: row tiles per (sequence, kv head), rows kept per record, key splits
+// attention_paged.hip: up to 16 rows (query rows x group) per sequence and kv head.  row tiles per (sequence, kv head), rows
+// kept per record, key splits
 struct StepShape {
     int row_tiles, rows, splits;
 };
-StepShape step_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
+StepShape step_shape(size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
                      bool one_row_each);
-hipError_t launch_attention_paged(int head_dim, const PagedAttnArgs& a, const StepShape& s, hipStream_t st);
-hipError_t launch_attention_ragged(int head_dim, const PagedAttnArgs& a, hipStream_t st);
+hipError_t launch_attention_step(int head_dim, const PagedAttnArgs& a, const StepShape& s, hipStream_t st);
+// attention_tiles.hip: 128 rows at a time, over the pages or over FP16 rows
+struct TileShape {
+    int slots, splits;
+};
+TileShape tile_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink);
+size_t tile_record_floats(size_t head_dim);
+hipError_t launch_attention_tiles(int head_dim, bool paged, const PagedAttnArgs& a, const TileShape& s, hipStream_t st);
 
 }  // namespace cactus_hip

@@ -50,4 +50,18 @@ __device__ __forceinline__ int page_of(const PagedCache& c, int b, int i) {
     return p >= 0 && p < c.num_pages ? p : -1;
 }
 
+// The key tiles that rows at positions first .. last see: `sinks` tiles from key 0, then tile `first` and on.
+struct TilePlan {
+    int sinks, first, tiles;
+};
+__device__ __forceinline__ TilePlan plan_tiles(int pos_first, int pos_last, int window, int sink, int size) {
+    TilePlan p;
+    const int all = pos_last < 0 ? 0 : pos_last / size + 1;
+    const int low = window ? pos_first - window : 0;
+    p.first = low > 0 ? low / size : 0;
+    p.sinks = min(p.first, window ? (sink + size - 1) / size : 0);
+    p.tiles = p.sinks + max(all - p.first, 0);
+    return p;
+}
+
 }  // namespace cactus_hip

@@ -74,6 +74,10 @@ const char* bad_window(size_t window, size_t sink) {
     return window > 0x7fffffff || sink > 0x7fffffff ? "window and sink must be below 2^31" : nullptr;
 }
 
+// Positions lie below 2^30 (a table holds at most 2^30 tokens): a larger window or sink sees the same, and differences of two
+// of them stay in an int.
+int reach(size_t n) { return n < (size_t(1) << 30) ? (int)n : 1 << 30; }
+
 PagedCache view(const cactus_hip_paged_kv& c, const int32_t* tables, size_t width) {
     PagedCache v{};
     v.k = c.k;
@@ -86,6 +90,36 @@ PagedCache view(const cactus_hip_paged_kv& c, const int32_t* tables, size_t widt
     v.page_shift = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : c.page_size == 64 ? 6 : 7;
     v.kv_heads = (int)c.kv_heads;
     return v;
+}
+
+// How a call of the paged attention is cut.  One row per sequence: the step kernel.  A ragged batch: sequences of at most 16
+// rows per kv head are the step kernel's, longer ones the tile kernel's; which of them a batch holds only the device knows, so
+// both are launched - except when the average is 64 rows or more (a batch of prompt chunks), where an odd short sequence
+// costs less in the tile kernel than a launch that finds nothing to do (about 3 us).
+struct PagedPlan {
+    bool by_step, by_tile;
+    StepShape step;
+    TileShape tile;
+    size_t step_items, tile_items, step_bytes, tile_bytes;
+    size_t bytes() const { return step_bytes + tile_bytes; }
+    size_t items() const { return step_items > tile_items ? step_items : tile_items; }
+};
+PagedPlan paged_plan(const cactus_hip_paged_kv& c, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t window,
+                     size_t sink, bool one_row_each) {
+    PagedPlan p{};
+    p.by_step = one_row_each || tokens * (q_heads / c.kv_heads) < 64 * batch;
+    p.by_tile = !one_row_each;
+    if (p.by_step) {
+        p.step = step_shape(batch, max_context, q_heads, c.kv_heads, window, sink, one_row_each);
+        p.step_items = batch * c.kv_heads * p.step.row_tiles * p.step.splits;
+        if (p.step.splits > 1) p.step_bytes = p.step_items * p.step.rows * (c.head_dim + 2) * sizeof(float);
+    }
+    if (p.by_tile) {
+        p.tile = tile_shape(batch, tokens, max_context, q_heads, c.kv_heads, window, sink);
+        p.tile_items = (size_t)p.tile.slots * c.kv_heads * p.tile.splits;
+        if (p.tile.splits > 1) p.tile_bytes = p.tile_items * tile_record_floats(c.head_dim) * sizeof(float);
+    }
+    return p;
 }
 
 // theta^(-2i/D) / (2 pi) for the pairs of a head; a decode loop asks for the same two numbers every step
@@ -172,9 +206,9 @@ int cactus_hip_kv_read_paged_f16_dev(const cactus_hip_paged_kv* cache, const int
 size_t cactus_hip_attention_paged_workspace_bytes(const cactus_hip_paged_kv* cache, size_t batch, size_t tokens,
                                                   size_t max_context, size_t num_q_heads, size_t window, size_t sink,
                                                   int one_row_each) {
-    if (!cache || batch == 0 || tokens == 0 || bad_groups(num_q_heads, cache->kv_heads) || batch > MAX_BATCH) return 0;
-    const StepShape s = step_shape(batch, tokens, max_context, num_q_heads, cache->kv_heads, window, sink, one_row_each != 0);
-    return s.splits == 1 ? 0 : batch * cache->kv_heads * s.row_tiles * s.splits * s.rows * (cache->head_dim + 2) * sizeof(float);
+    if (!cache || batch == 0 || tokens == 0 || bad_groups(num_q_heads, cache->kv_heads) || batch > MAX_BATCH || tokens > MAX_ROWS)
+        return 0;
+    return paged_plan(*cache, batch, tokens, max_context, num_q_heads, window, sink, one_row_each != 0).bytes();
 }
 
 int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const int32_t* block_tables, size_t table_width,
@@ -204,16 +238,22 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
     a.q_heads = (int)num_q_heads;
     a.kv_heads = (int)cache->kv_heads;
     a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)cache->head_dim) : scale;
-    a.window = (int)window;
-    a.sink = (int)sink;
-    const size_t need = cactus_hip_attention_paged_workspace_bytes(cache, batch, tokens, max_context, num_q_heads, window, sink,
-                                                                   cu_seqlens == nullptr);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    a.window = reach(window);
+    a.sink = reach(sink);
+    const PagedPlan p = paged_plan(*cache, batch, tokens, max_context, num_q_heads, window, sink, cu_seqlens == nullptr);
+    if (p.bytes() > 0 && (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace)))
         return refuse(who, "workspace missing, too small or not 16-byte aligned");
-    const StepShape s = step_shape(batch, tokens, max_context, num_q_heads, cache->kv_heads, window, sink, cu_seqlens == nullptr);
+    if (p.items() > 0x7fffffff) return refuse(who, "too many rows for one launch");
     a.work = static_cast<float*>(workspace);
-    a.work_rows = s.rows;
-    return launched(who, launch_attention_paged((int)cache->head_dim, a, s, (hipStream_t)stream));
+    if (p.by_step) {
+        a.work_rows = p.step.rows;
+        const int rc = launched(who, launch_attention_step((int)cache->head_dim, a, p.step, (hipStream_t)stream));
+        if (rc != CACTUS_HIP_OK) return rc;
+        a.work += p.step_bytes / sizeof(float);
+        a.min_rows = 16;
+    }
+    if (p.by_tile) return launched(who, launch_attention_tiles((int)cache->head_dim, true, a, p.tile, (hipStream_t)stream));
+    return CACTUS_HIP_OK;
 }
 
 int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride, const cactus_half_t* k, size_t k_stride,
@@ -247,9 +287,11 @@ int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride,
     a.q_heads = (int)num_q_heads;
     a.kv_heads = (int)num_kv_heads;
     a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)head_dim) : scale;
-    a.window = (int)window;
-    a.sink = (int)sink;
-    return launched(who, launch_attention_ragged((int)head_dim, a, (hipStream_t)stream));
+    a.window = reach(window);
+    a.sink = reach(sink);
+    const TileShape s = {tile_shape(batch, tokens, 0, num_q_heads, num_kv_heads, window, sink).slots, 1};
+    if ((size_t)s.slots * num_kv_heads > 0x7fffffff) return refuse(who, "too many rows for one launch");
+    return launched(who, launch_attention_tiles((int)head_dim, false, a, s, (hipStream_t)stream));
 }
 
 }  // extern "C"

@@ -62,10 +62,13 @@ def seen(position, keys, window, sink):
     return ok
 
 
-def attend(q, k, v, positions, window, sink, scale=0.0, extra=None):
+def attend(q, k, v, positions, window, sink, scale=0.0, extra=None, ratio=1.0):
     """q [n, Hq, D], k / v [L, Hkv, D] -> (out, bound) [n, Hq, D].  extra [L]: keys that can be seen at all.
     The bound: the output's rounding; every weight rounded to binary16; scores in fp32 (D products, the scale, the base-2
-    argument: D + 8 roundings of the sum of |q k|), which enter numerator and denominator; fp32 sums over L keys."""
+    argument: D + 8 roundings of the sum of |q k|), which enter numerator and denominator; fp32 sums over L keys.
+    Binary16 is subnormal below 2^-14: a weight that small beside the largest is rounded by 2^-25 of the largest, however
+    small it is.  ratio: how far the page scales of the values lie apart; a weight is rounded together with its page's scale,
+    so beside the largest it may be that much smaller, and its value that much larger."""
     n, Hq, D = q.shape
     L, Hkv, _ = k.shape
     scale = scale or 1 / math.sqrt(D)
@@ -88,6 +91,8 @@ def attend(q, k, v, positions, window, sink, scale=0.0, extra=None):
             weighted = w @ vv[:, hk].abs()
             delta = (D + 8) * U32 * mag
             tol[i, h] = U16 * out[i, h].abs() + weighted * (U16 + 2 * delta + (int(ok.sum()) + 16) * U32) + 2.0 ** -24
+            small = w < w.max() * ratio * 2.0 ** -14
+            tol[i, h] += 2.0 ** -25 * w.max() * ratio * vv[small][:, hk].abs().sum(0)
     return out, tol
 
 

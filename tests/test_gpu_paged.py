@@ -240,6 +240,12 @@ def test_read(P, D, Hkv, page):
 
 # ---------------------------------------------------------------------------------------------------- paged attention
 
+def spread(scales):
+    """How far the scales of written pages lie apart."""
+    s = scales[scales > 0]
+    return float(s.max() / s.min()) if s.numel() else 1.0
+
+
 def check_attention(P, seed, D, page, Hq, Hkv, news, contexts, window=0, sink=0, use_cu=True, scale=0.0, edit=None, width=None,
                     max_context=None, strided=False, qscale=1.5):
     gen = torch.Generator().manual_seed(seed)
@@ -270,7 +276,7 @@ def check_attention(P, seed, D, page, Hq, Hkv, news, contexts, window=0, sink=0,
         k, ok = R.gather(kv[0], kv[2], tables[b], page, 0, c)
         v, _ = R.gather(kv[1], kv[3], tables[b], page, 0, c)
         r = slice(int(cu[b]), int(cu[b]) + n)
-        want, tol = R.attend(q[r], k, v, torch.arange(c - n, c), window, sink, scale, ok)
+        want, tol = R.attend(q[r], k, v, torch.arange(c - n, c), window, sink, scale, ok, spread(kv[3]))
         err = (out[r].cpu().double() - want).abs()
         assert bool((err <= tol).all()), (b, n, c, float((err / tol).max()))
         worst = max(worst, float((err / tol).max()) if err.numel() else 0.0)
@@ -558,7 +564,7 @@ def test_prompt_then_tokens(P, D, Hq, Hkv, page, window, sink):
             kk, _ = R.gather(kv[0].cpu(), kv[2].cpu(), tables[b], page, 0, c)
             vv, _ = R.gather(kv[1].cpu(), kv[3].cpu(), tables[b], page, 0, c)
             assert read_back(back[0][rd:rd + c], kk) and read_back(back[1][rd:rd + c], vv)
-            want, tol = R.attend(qr[at:at + n].cpu(), kk, vv, torch.arange(have[b], c), window, sink)
+            want, tol = R.attend(qr[at:at + n].cpu(), kk, vv, torch.arange(have[b], c), window, sink, ratio=spread(kv[3].cpu()[tables[b].long()]))
             assert bool(((out[at:at + n].cpu().double() - want).abs() <= tol).all())
             # the newest rows are in the cache to within half a step of their page's scale
             x, terms = R.norm_rope(k[at:at + n].cpu(), kw, eps, theta, torch.arange(have[b], c))
