@@ -81,6 +81,10 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     __shared__ __attribute__((aligned(1024))) unsigned char s_k[2][BK * ROW];
     __shared__ __attribute__((aligned(1024))) unsigned char s_v[2][BK * ROW];
     __shared__ float s_scale[2][GROUPS][2];
+    // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
+    // tile, not seen whole by every row, that holds such values; s_marks: +inf, -inf, NaN bits of every row's dims
+    __shared__ int s_odd[2];
+    __shared__ uint32_t s_marks[PAGED ? 1 : 3][PAGED ? 1 : TILE_ROWS][D / 32];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
@@ -163,7 +167,28 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             }
         }
     };
-    const auto stash = [&](const Load& t, int buf) {
+    const auto stash = [&](Load& t, int u, int buf) {
+        if constexpr (!PAGED) {
+            const int key = key_of(u);
+            if (key + BK - 1 > pos_of(0) || (a.window && key < last - a.window && key + BK > a.sink)) {
+                uint32_t odd = 0;
+#pragma unroll
+                for (int i = 0; i < Load::PIECES; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) odd |= (((uint32_t)t.v[i][e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                if (odd) {
+                    s_odd[buf] = u + 1;
+#pragma unroll
+                    for (int i = 0; i < Load::PIECES; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t x = (uint32_t)t.v[i][e];
+                            t.v[i][e] = (int)(((x & 0x7c00u) == 0x7c00u ? 0u : x & 0xffffu) |
+                                              ((x & 0x7c000000u) == 0x7c000000u ? 0u : x & 0xffff0000u));
+                        }
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < Load::PIECES; i++) {
             const int p = i * 256 + tid;
@@ -203,8 +228,14 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 
     // lane addresses: K row n of a 32-key half, chunk 2 s + h; V key 4 h + tq, dims 16 (gi & 1) + 4 tp .. of a 32-dim tile
     const int tq = (lane >> 2) & 3, tp = lane & 3, gi = (lane >> 4) & 1;
-    const auto compute = [&](auto whole_tag, int u, int buf) __attribute__((always_inline)) {
-        constexpr bool WHOLE = decltype(whole_tag)::value;
+    // the eight keys of group g that a lane holds for its dim of 32-dim tile i
+    const auto value_frag = [&](int buf, int i, int g) __attribute__((always_inline)) {
+        const unsigned char* at = s_v[buf] + (16 * g + 4 * h + tq) * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
+        const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
+        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * ROW));
+        return __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+    };
+    const auto compute = [&](int u, int buf, bool whole) __attribute__((always_inline)) {
         const int key = key_of(u);
         v16f s[KT];
 #pragma unroll
@@ -230,13 +261,15 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 for (int r = 0; r < 8; r++) s[g >> 1][8 * (g & 1) + r] = fmaf(s[g >> 1][8 * (g & 1) + r], up, add);
             }
         }
-        if constexpr (!WHOLE) {
+        if (!whole) {
+            // key 32 t + 8 (r / 4) + 4 h + r % 4 of the tile, against this row's last key, first window key and sinks
+            const int to = pos - key - 4 * h, from = a.window ? to - a.window : -BK, sinks = a.sink - key - 4 * h;
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int j = key + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
-                    bool seen = j <= pos && (!a.window || pos - j <= a.window || j < a.sink);
+                    const int j = 32 * t + 8 * (r >> 2) + (r & 3);
+                    bool seen = j <= to && (j >= from || j < sinks);
                     if constexpr (PAGED) seen = seen && live[2 * t + (r >> 3)];
                     s[t][r] = seen ? s[t][r] : -INFINITY;
                 }
@@ -278,42 +311,35 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
         for (int i = 0; i < NDT; i++)
 #pragma unroll
-            for (int g = 0; g < GROUPS; g++) {
-                const int r = 16 * g + 4 * h + tq;
-                const unsigned char* at = s_v[buf] + r * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
-                const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
-                const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * ROW));
-                v8h vf = __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
-                if constexpr (!PAGED && !WHOLE) {
-                    // a value that is not finite must not reach a row that does not see its key: 0 * inf is NaN
-                    const v4i x = __builtin_bit_cast(v4i, vf);
-                    uint32_t odd = 0;
+            for (int g = 0; g < GROUPS; g++)
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value_frag(buf, i, g), p[g], o[i], 0, 0, 0);
+        if constexpr (!PAGED) {
+            if (s_odd[buf] == u + 1) {
+                // The values that are not finite are zero in LDS (stash).  Every row that puts weight on such a key is marked:
+                // the output of that dim becomes what adding the value makes of it.
+                uint32_t mine = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) odd |= (((uint32_t)x[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
-                    if (__any(odd != 0)) {
-                        // the weights of +inf, -inf and NaN values of a dim are summed apart: any weight there is the result
-                        v8u y = __builtin_bit_cast(v8u, vf), mark;
+                for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) mine |= p[g][e] > (_Float16)0.0f || p[g][e] != p[g][e] ? 1u << (8 * g + e) : 0u;
+                const uint32_t other = __shfl_xor(mine, 32);
 #pragma unroll 1
-                        for (int kind = 0; kind < 3; kind++) {
-                            const uint16_t lo = kind == 0 ? 0x7c00u : kind == 1 ? 0xfc00u : 0x7c01u;
-#pragma unroll
-                            for (int e = 0; e < 8; e++)
-                                mark[e] = (kind < 2 ? y[e] == lo : (y[e] & 0x7fffu) >= lo) ? 0x3c00u : 0u;     // 1 or 0
-                            v16f sum;
-#pragma unroll
-                            for (int r2 = 0; r2 < 16; r2++) sum[r2] = 0.0f;
-                            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, mark), p[g], sum, 0, 0, 0);
-                            const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-#pragma unroll
-                            for (int r2 = 0; r2 < 16; r2++) o[i][r2] += sum[r2] > 0.0f ? add : 0.0f;
+                for (int k = 0; k < BK && key + k <= last; k++) {
+                    const int bit = 8 * (k >> 4) + 4 * ((k >> 3) & 1) + (k & 3);
+                    const bool weighed = (((((k >> 2) & 1) == h ? mine : other) >> bit) & 1) != 0;
+#pragma unroll 1
+                    for (int d0 = 0; d0 < D; d0 += 64) {
+                        const uint32_t x = a.v[(size_t)(rows.first + key + k) * a.v_stride + (size_t)head * D + d0 + lane];
+                        for (unsigned long long odd = __ballot((x & 0x7c00u) == 0x7c00u); odd; odd &= odd - 1) {
+                            const int at = __builtin_ctzll(odd), d = d0 + at;
+                            const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)x, at);
+                            const int kind = y == 0x7c00u ? 0 : y == 0xfc00u ? 1 : 2;
+                            if (weighed) atomicOr(&s_marks[kind][wave * 32 + n][d >> 5], 1u << (d & 31));
                         }
-#pragma unroll
-                        for (int e = 0; e < 8; e++) y[e] = (y[e] & 0x7c00u) == 0x7c00u ? 0 : y[e];
-                        vf = __builtin_bit_cast(v8h, y);
                     }
                 }
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[g], o[i], 0, 0, 0);
             }
+        }
     };
 
     if (u0 < u1) {
@@ -321,7 +347,12 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         look_up(u0);
         fetch(t, u0);
         look_up(u0 + 1);
-        stash(t, 0);
+        if constexpr (!PAGED) {
+            if (tid < 2) s_odd[tid] = 0;
+            for (int i = tid; i < 3 * TILE_ROWS * (D / 32); i += 256) (&s_marks[0][0][0])[i] = 0;
+            __syncthreads();
+        }
+        stash(t, u0, 0);
         __syncthreads();
         for (int u = u0, buf = 0; u < u1; u++, buf ^= 1) {
             if (u + 1 < u1) {
@@ -336,12 +367,9 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                     for (int g = 0; g < GROUPS; g++) whole = whole && s_scale[buf][g][1] >= 0.0f;
                     whole = __builtin_amdgcn_readfirstlane(whole);
                 }
-                if (whole)
-                    compute(std::true_type{}, u, buf);
-                else
-                    compute(std::false_type{}, u, buf);
+                compute(u, buf, whole);
             }
-            if (u + 1 < u1) stash(t, buf ^ 1);
+            if (u + 1 < u1) stash(t, u + 1, buf ^ 1);
             __syncthreads();
         }
     }
@@ -374,7 +402,16 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             for (int r = 0; r < 16; r += 4) {
                 v4h x;
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = (_Float16)(o[i][r + e] * inv);
+                for (int e = 0; e < 4; e++) {
+                    float y = o[i][r + e] * inv;
+                    if constexpr (!PAGED) {
+                        const int at = 2 * r + 4 * h + e;            // of 32-dim tile i
+                        y += (s_marks[0][wave * 32 + n][i] >> at) & 1 ? INFINITY : 0.0f;
+                        y += (s_marks[1][wave * 32 + n][i] >> at) & 1 ? -INFINITY : 0.0f;
+                        y += (s_marks[2][wave * 32 + n][i] >> at) & 1 ? NAN : 0.0f;
+                    }
+                    x[e] = (_Float16)y;
+                }
                 *reinterpret_cast<v4h*>(out + 32 * i + 2 * r + 4 * h) = x;
             }
     }
