@@ -73,6 +73,13 @@ struct TileLoad {
     float scale;         // lane 2 g + (0 key, 1 value) of the first wave: the scale of 16-key group g
 };
 
+// Launch order of the slots.  A causal tile's work grows with its position, so late slots go first; when the chip holds the whole
+// launch at two workgroups per CU, the second half goes the other way, so that the two of a CU add up to the same work.
+__device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
+    const int half = (slots + 1) / 2;
+    return slots * kv_heads > 512 || rank < half ? slots - 1 - rank : rank - half;
+}
+
 template <int D, bool PAGED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int slots) {
@@ -89,7 +96,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     // kv heads go round first (a head's rows stay in one XCD's L2 when their number divides by 8), heavy slots early
-    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads;
+    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
     const int group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
@@ -421,7 +428,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 template <int D>
 __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int splits, const int slots) {
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = blockIdx.x, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads, group = a.q_heads / a.kv_heads;
+    const int id = blockIdx.x, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads), group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
     const Rows rows = rows_of(a.cu, b, a.tokens);
@@ -464,7 +471,8 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 // as many as fill it twice over, each with at least 512 keys.
 TileShape tile_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink) {
     TileShape s;
-    s.slots = (int)(tokens * (q_heads / kv_heads) / TILE_ROWS + batch);
+    const size_t rows = tokens * (q_heads / kv_heads);
+    s.slots = (int)(batch == 1 ? (rows + TILE_ROWS - 1) / TILE_ROWS : rows / TILE_ROWS + batch);     // slot_begin
     const size_t items = (size_t)s.slots * kv_heads;
     size_t keys = max_context;
     if (window && window + sink + TILE_ROWS < keys) keys = window + sink + TILE_ROWS;

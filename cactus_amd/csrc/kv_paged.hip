@@ -4,12 +4,13 @@
 // max(|x|) / 127 of its tokens, q = rne(x / scale).  Bound: HBM for prompts (rows in, INT8 and the q rows out: every byte
 // moves once), launch latency for a decode step.
 //
-// A workgroup takes the part of ONE page that the call writes, for some kv heads and their query heads, so that a page's
-// maximum never leaves the workgroup.  D / 16 lanes hold a row: lane j the 8 elements from 8 j and their rotation partners
-// from D / 2 + 8 j, two 16-byte loads, no exchange for the rotation.  The row slots of a workgroup are split into
-// (token of the page) x (head): STEP (one row per sequence) gives them all to heads, otherwise tokens come first.  A lane
-// keeps its tokens while it walks the heads, so an angle is computed once per workgroup and not once per head: in fp64 as
-// turns (pos * theta^(-2i/D) / 2 pi, only the fraction kept), because an fp32 product at position 30000 is off by 1e-3.
+// A workgroup takes the part of ONE page that the call writes, either for some kv heads (keys and values: a page's maximum
+// never leaves the workgroup) or for some query heads; the launch cuts the heads finer the fewer pages there are.  D / 16 lanes
+// hold a row: lane j the 8 elements from 8 j and their rotation partners from D / 2 + 8 j, two 16-byte loads, no exchange for
+// the rotation.  The row slots of a workgroup are (token of the page) x (head): STEP (one row per sequence) gives them all to
+// heads, otherwise tokens come first.  A lane keeps its tokens while it walks the heads, so an angle is computed once per
+// workgroup: in fp64 as turns (pos * theta^(-2i/D) / 2 pi, only the fraction kept), because an fp32 product at position 30000
+// is off by 1e-3; v_sin_f32 / v_cos_f32 take turns and are off by 2^-23 at most (measured).
 #include "paged.hip.h"
 
 #include <math.h>
@@ -84,13 +85,20 @@ __device__ __forceinline__ float absmax(const Row16& r) {
     return m;
 }
 
+// x / scale rounded to an integer, as a byte.  |x| <= 127 scale.  One step of refinement makes the product with the reciprocal the
+// quotient: without it one value in 10^5 falls on the other side of a half.
+__device__ __forceinline__ uint32_t code(float x, float scale, float inv) {
+    const float y = x * inv;
+    return (uint32_t)rne_i32(fmaf(fmaf(-y, scale, x), inv, y)) & 0xFFu;
+}
 template <int D>
-__device__ __forceinline__ void store_i8(int8_t* __restrict__ row, int j, const Row16& r, float inv) {
+__device__ __forceinline__ void store_i8(int8_t* __restrict__ row, int j, const Row16& r, float scale) {
+    const float inv = 1.0f / scale;
     uint32_t o[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        o[e >> 2] |= (uint32_t)(clamp_i8(rne_i32(r.lo[e] * inv)) & 0xFF) << (8 * (e & 3));
-        o[2 + (e >> 2)] |= (uint32_t)(clamp_i8(rne_i32(r.hi[e] * inv)) & 0xFF) << (8 * (e & 3));
+        o[e >> 2] |= code(r.lo[e], scale, inv) << (8 * (e & 3));
+        o[2 + (e >> 2)] |= code(r.hi[e], scale, inv) << (8 * (e & 3));
     }
     *reinterpret_cast<uint2*>(row + 8 * j) = make_uint2(o[0], o[1]);
     *reinterpret_cast<uint2*>(row + D / 2 + 8 * j) = make_uint2(o[2], o[3]);
@@ -101,9 +109,9 @@ constexpr int MAX_SLOTS = 256;   // row slots of a workgroup (1024 threads, 4 la
 template <int D, bool STEP>
 __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArgs a) {
     constexpr int LPR = D / 16;
-    constexpr int RPL = STEP ? 1 : 2;     // tokens a lane holds: the launch picks the workgroup so that 2 are enough
-    __shared__ uint32_t s_max[2][MAX_SLOTS];
-    __shared__ float s_again[2][MAX_SLOTS];      // old / new scale of a head whose earlier tokens are requantized, else 0
+    constexpr int RPL = STEP ? 1 : 2;            // tokens a lane holds: the launch picks the workgroup so that 2 are enough
+    __shared__ uint32_t s_max[MAX_SLOTS];
+    __shared__ float s_again[MAX_SLOTS];         // old / new scale of a head whose earlier tokens are requantized, else -1
 
     const int tid = threadIdx.x, slot = tid / LPR, j = tid % LPR, slots = blockDim.x / LPR;
     const int P = 1 << a.c.page_shift;
@@ -124,7 +132,6 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
     if (base >= pos0 + rows.count) return;
     const int e_lo = (int)max(pos0 - base, 0LL), e_hi = (int)min(pos0 + rows.count - base, (long long)P);
     const int row0 = rows.first + (int)(base - pos0);          // packed row of page slot 0
-    const int page = index < a.c.table_width ? page_of(a.c, b, (int)index) : -1;
 
     const int TP = STEP ? 1 : min(P, slots), HP = slots / TP;  // tokens x heads of a pass
     const int ts = slot % TP, hs = slot / TP;
@@ -140,109 +147,24 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const double t = pos * a.rope.turn[8 * j + i];
-                sincospif(2.0f * (float)(t - floor(t)), &sn[r][i], &cs[r][i]);
+                const float turn = (float)(t - rint(t));
+                sn[r][i] = __builtin_amdgcn_sinf(turn);
+                cs[r][i] = __builtin_amdgcn_cosf(turn);
             }
         }
     }
 
-    const int kv0 = blockIdx.y * a.kv_per_group, kvn = min(a.kv_per_group, a.c.kv_heads - kv0);
-    Row16 kw{}, qw{};
-    if (a.k_weight) kw = load_row<D>(a.k_weight, j);
-    if (a.q_weight) qw = load_row<D>(a.q_weight, j);
-
-    if (page >= 0) {
-        for (int h0 = 0; h0 < kvn; h0 += HP) {
-            const int h = kv0 + h0 + hs;
-            const bool head = h0 + hs < kvn;
-            const size_t ph = (size_t)page * a.c.kv_heads + h;
-            float old_k = 0.0f, old_v = 0.0f;
-            if (head && e_lo > 0) {
-                old_k = a.c.ks[ph];
-                old_v = a.c.vs[ph];
-            }
-            if constexpr (!STEP) {
-                for (int i = tid; i < 2 * MAX_SLOTS; i += blockDim.x) (&s_max[0][0])[i] = 0;
-                __syncthreads();
-            }
-            Row16 kr[RPL], vr[RPL];
-            float mk = 0.0f, mv = 0.0f;
-#pragma unroll
-            for (int r = 0; r < RPL; r++) {
-                if (!head || !live[r]) continue;     // the same for all lanes of a row
-                const size_t row = (size_t)(row0 + e[r]);
-                kr[r] = load_row<D>(a.k + row * a.k_stride + (size_t)h * D, j);
-                vr[r] = load_row<D>(a.v + row * a.v_stride + (size_t)h * D, j);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    kr[r].lo[i] = finite_half(kr[r].lo[i]);
-                    kr[r].hi[i] = finite_half(kr[r].hi[i]);
-                    vr[r].lo[i] = finite_half(vr[r].lo[i]);
-                    vr[r].hi[i] = finite_half(vr[r].hi[i]);
-                }
-                norm_rotate<D>(kr[r], a.k_weight != nullptr, kw, a.eps, a.rotate, cs[r], sn[r]);
-                mk = fmaxf(mk, absmax(kr[r]));
-                mv = fmaxf(mv, absmax(vr[r]));
-            }
-            mk = row_max<LPR>(mk);
-            mv = row_max<LPR>(mv);
-            if constexpr (!STEP) {
-                if (j == 0 && head) {   // bits of non-negative floats order as the floats do: the maximum is the same in any order
-                    atomicMax(&s_max[0][hs], __float_as_uint(mk));
-                    atomicMax(&s_max[1][hs], __float_as_uint(mv));
-                }
-                __syncthreads();
-                mk = __uint_as_float(s_max[0][hs]);
-                mv = __uint_as_float(s_max[1][hs]);
-            }
-            const float new_k = fmaxf(old_k, fmaxf(mk / 127.0f, 1e-10f)), new_v = fmaxf(old_v, fmaxf(mv / 127.0f, 1e-10f));
-            const float inv_k = 1.0f / new_k, inv_v = 1.0f / new_v;
-#pragma unroll
-            for (int r = 0; r < RPL; r++) {
-                if (!head || !live[r]) continue;
-                const size_t at = (ph << a.c.page_shift) + e[r];
-                store_i8<D>(a.c.k + at * D, j, kr[r], inv_k);
-                store_i8<D>(a.c.v + at * D, j, vr[r], inv_v);
-            }
-            if (head && ts == 0 && j == 0) {
-                a.c.ks[ph] = new_k;
-                a.c.vs[ph] = new_v;
-                s_again[0][hs] = e_lo > 0 && new_k > old_k ? old_k / new_k : -1.0f;
-                s_again[1][hs] = e_lo > 0 && new_v > old_v ? old_v / new_v : -1.0f;
-            }
-            if (e_lo > 0) {             // the page held tokens before: bring them to a scale that has grown
-                __syncthreads();
-                for (int w = 0; w < 2 * min(HP, kvn - h0); w++) {
-                    const float f = s_again[w & 1][w >> 1];
-                    if (f < 0.0f) continue;
-                    const size_t first = (((size_t)page * a.c.kv_heads + kv0 + h0 + (w >> 1)) << a.c.page_shift) * D;
-                    int8_t* x = ((w & 1) ? a.c.v : a.c.k) + first;
-                    for (int i = tid * 16; i < e_lo * D; i += blockDim.x * 16) {
-                        v4i q = *reinterpret_cast<const v4i*>(x + i);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            uint32_t o = 0;
-#pragma unroll
-                            for (int s = 0; s < 4; s++)
-                                o |= (uint32_t)(rne_i32((float)(int8_t)((uint32_t)q[c] >> (8 * s)) * f) & 0xFF) << (8 * s);
-                            q[c] = (int)o;
-                        }
-                        *reinterpret_cast<v4i*>(x + i) = q;
-                    }
-                }
-            }
-            __syncthreads();
-        }
-    }
-
-    if (a.q) {
-        const int g = a.q_heads / a.c.kv_heads, q0 = kv0 * g, qn = kvn * g;
+    if ((int)blockIdx.y >= a.kv_parts) {         // query heads
+        Row16 w{};
+        if (a.q_weight) w = load_row<D>(a.q_weight, j);
+        const int q0 = ((int)blockIdx.y - a.kv_parts) * a.q_per_part, qn = min(a.q_per_part, a.q_heads - q0);
         for (int h0 = hs; h0 < qn; h0 += HP) {
 #pragma unroll
             for (int r = 0; r < RPL; r++) {
-                if (!live[r]) continue;
+                if (!live[r]) continue;          // the same for all lanes of a row
                 const size_t row = (size_t)(row0 + e[r]);
                 Row16 x = load_row<D>(a.q + row * a.q_stride + (size_t)(q0 + h0) * D, j);
-                norm_rotate<D>(x, a.q_weight != nullptr, qw, a.eps, a.rotate, cs[r], sn[r]);
+                norm_rotate<D>(x, a.q_weight != nullptr, w, a.eps, a.rotate, cs[r], sn[r]);
                 v8h lo, hi;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -254,6 +176,80 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
                 *reinterpret_cast<v8h*>(out + D / 2 + 8 * j) = hi;
             }
         }
+        return;
+    }
+
+    const int page = index < a.c.table_width ? page_of(a.c, b, (int)index) : -1;
+    if (page < 0) return;
+    const int kv0 = blockIdx.y * a.kv_per_part, kvn = min(a.kv_per_part, a.c.kv_heads - kv0);
+    Row16 w{};
+    if (a.k_weight) w = load_row<D>(a.k_weight, j);
+    // items: the keys of kvn heads, then their values
+    for (int i0 = 0; i0 < 2 * kvn; i0 += HP) {
+        const int item = i0 + hs;
+        const bool on = item < 2 * kvn, value = item >= kvn;
+        const size_t ph = (size_t)page * a.c.kv_heads + kv0 + (value ? item - kvn : item);
+        float* scale = (value ? a.c.vs : a.c.ks) + ph;
+        const float old = on && e_lo > 0 ? *scale : 0.0f;
+        if constexpr (!STEP) {
+            for (int i = tid; i < HP; i += blockDim.x) s_max[i] = 0;
+            __syncthreads();
+        }
+        Row16 x[RPL];
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < RPL; r++) {
+            if (!on || !live[r]) continue;
+            const size_t row = (size_t)(row0 + e[r]), head = (size_t)(kv0 + (value ? item - kvn : item)) * D;
+            x[r] = load_row<D>((value ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head, j);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[r].lo[i] = finite_half(x[r].lo[i]);
+                x[r].hi[i] = finite_half(x[r].hi[i]);
+            }
+            if (!value) norm_rotate<D>(x[r], a.k_weight != nullptr, w, a.eps, a.rotate, cs[r], sn[r]);
+            top = fmaxf(top, absmax(x[r]));
+        }
+        top = row_max<LPR>(top);
+        if constexpr (!STEP) {
+            // bits of non-negative floats order as the floats do: the maximum is the same in any order
+            if (j == 0 && on) atomicMax(&s_max[hs], __float_as_uint(top));
+            __syncthreads();
+            top = __uint_as_float(s_max[hs]);
+        }
+        const float now = fmaxf(old, fmaxf(top / 127.0f, 1e-10f));
+#pragma unroll
+        for (int r = 0; r < RPL; r++) {
+            if (!on || !live[r]) continue;
+            store_i8<D>((value ? a.c.v : a.c.k) + ((ph << a.c.page_shift) + e[r]) * D, j, x[r], now);
+        }
+        if (on && ts == 0 && j == 0) {
+            *scale = now;
+            s_again[hs] = now > old ? old / now : -1.0f;
+        }
+        if (e_lo > 0) {                          // the page held tokens before: bring them to a scale that has grown
+            __syncthreads();
+            for (int c = 0; c < min(HP, 2 * kvn - i0); c++) {
+                const float f = s_again[c];
+                if (f < 0.0f) continue;
+                const bool val = i0 + c >= kvn;
+                const size_t first = (((size_t)page * a.c.kv_heads + kv0 + (val ? i0 + c - kvn : i0 + c)) << a.c.page_shift) * D;
+                int8_t* codes = (val ? a.c.v : a.c.k) + first;
+                for (int i = tid * 16; i < e_lo * D; i += blockDim.x * 16) {
+                    v4i q = *reinterpret_cast<const v4i*>(codes + i);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t o = 0;
+#pragma unroll
+                        for (int s = 0; s < 4; s++)
+                            o |= (uint32_t)(rne_i32((float)(int8_t)((uint32_t)q[k] >> (8 * s)) * f) & 0xFF) << (8 * s);
+                        q[k] = (int)o;
+                    }
+                    *reinterpret_cast<v4i*>(codes + i) = q;
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -298,12 +294,24 @@ hipError_t append_paged(const PagedAppendArgs& args, hipStream_t st) {
     PagedAppendArgs a = args;
     const int P = 1 << a.c.page_shift, LPR = D / 16;
     const bool step = a.cu == nullptr;
-    // a workgroup per page piece and group of kv heads.  A step: 256 threads hold 256 / LPR heads at once.  Otherwise as
-    // many threads as let two tokens per lane cover a page.
+    // as many threads as let two tokens per lane cover a page; a step's row slots are its heads
     const int threads = step ? 256 : (P * LPR / 2 < 256 ? 256 : P * LPR / 2);
     const size_t pieces = step ? (size_t)a.batch : ((size_t)a.tokens >> a.c.page_shift) + 2 * (size_t)a.batch;
-    a.kv_per_group = a.c.kv_heads;
-    const dim3 grid((unsigned)pieces, (unsigned)((a.c.kv_heads + a.kv_per_group - 1) / a.kv_per_group));
+    // heads per workgroup: all of them when there are pages enough to fill the chip (about 1024 workgroups), one pass at least
+    const int at_once = step ? 256 / LPR : 1;
+    const auto cut = [&](int heads, int least) {
+        const size_t want = (1024 + pieces - 1) / pieces;
+        const int most = (heads + least - 1) / least, parts = want < (size_t)most ? (int)want : most;
+        return (heads + parts - 1) / parts;
+    };
+    a.kv_per_part = cut(a.c.kv_heads, at_once / 2 > 1 ? at_once / 2 : 1);
+    a.kv_parts = (a.c.kv_heads + a.kv_per_part - 1) / a.kv_per_part;
+    int q_parts = 0;
+    if (a.q) {
+        a.q_per_part = cut(a.q_heads, at_once);
+        q_parts = (a.q_heads + a.q_per_part - 1) / a.q_per_part;
+    }
+    const dim3 grid((unsigned)pieces, (unsigned)(a.kv_parts + q_parts));
     if (step)
         append_paged_kernel<D, true><<<grid, dim3(threads), 0, st>>>(a);
     else
