@@ -336,10 +336,12 @@ void attention_step_kernel(const PagedAttnArgs a, const int splits, const int ro
     }
 }
 
-// joins the splits of a row: one wave per row, lanes = dims
+// Joins the splits of a row: four waves per row, each every fourth split, lanes = dims; latency is all there is to it.
 template <int D>
-__global__ __launch_bounds__(64) void attention_join_kernel(const PagedAttnArgs a, const int splits, const int row_tiles) {
-    const int lane = threadIdx.x, item = blockIdx.x, rw = blockIdx.y;
+__global__ __launch_bounds__(256) void attention_join_kernel(const PagedAttnArgs a, const int splits, const int row_tiles) {
+    constexpr int W = D / 64;
+    __shared__ float s_l[4], s_o[4][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), item = blockIdx.x, rw = blockIdx.y;
     const int tile = item % row_tiles, head = item / row_tiles % a.kv_heads, b = item / row_tiles / a.kv_heads;
     const int group = a.q_heads / a.kv_heads;
     const Rows rows = rows_of(a.cu, b, a.tokens);
@@ -347,25 +349,29 @@ __global__ __launch_bounds__(64) void attention_join_kernel(const PagedAttnArgs 
     if (orow >= rows.count * group || (a.cu && rows.count * group > STEP_ROWS)) return;
     const size_t step = (size_t)a.work_rows * (D + 2);
     const float* rec = a.work + (size_t)item * splits * step;
-    float m = -1e30f, l = 0.0f;
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, rec[s * step + 2 * rw]);
-    m = wave_max(m);
-    constexpr int W = D / 64;
-    float o[W];
+    float m = -1e30f, l = 0.0f, o[W];
 #pragma unroll
     for (int i = 0; i < W; i++) o[i] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < splits; s++) {
+    for (int s = lane; s < splits; s += 64) m = fmaxf(m, rec[s * step + 2 * rw]);
+    m = wave_max(m);
+#pragma unroll 8
+    for (int s = wave; s < splits; s += 4) {
         const float f = __builtin_amdgcn_exp2f(rec[s * step + 2 * rw] - m);
         l = fmaf(rec[s * step + 2 * rw + 1], f, l);
         const float* x = rec + s * step + 2 * a.work_rows + rw * D + lane * W;
 #pragma unroll
         for (int i = 0; i < W; i++) o[i] = fmaf(x[i], f, o[i]);
     }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    uint16_t* out = a.out + ((size_t)(rows.first + orow / group) * a.q_heads + head * group + orow % group) * D + lane * W;
+    if (lane == 0) s_l[wave] = l;
 #pragma unroll
-    for (int i = 0; i < W; i++) out[i] = f2h(o[i] * inv);
+    for (int i = 0; i < W; i++) s_o[wave][lane * W + i] = o[i];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    a.out[((size_t)(rows.first + orow / group) * a.q_heads + head * group + orow % group) * D + d] =
+        f2h(((s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d])) * inv);
 }
 
 template <int D>
@@ -375,7 +381,7 @@ hipError_t launch_step(const PagedAttnArgs& a, const StepShape& s, hipStream_t s
                                (size_t)STEP_WAVES * s.rows * (D < 128 ? D : 128) * sizeof(float), st>>>(a, s.splits, s.row_tiles);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || s.splits == 1) return e;
-    attention_join_kernel<D><<<dim3((unsigned)items, (unsigned)s.rows), dim3(64), 0, st>>>(a, s.splits, s.row_tiles);
+    attention_join_kernel<D><<<dim3((unsigned)items, (unsigned)s.rows), dim3(256), 0, st>>>(a, s.splits, s.row_tiles);
     return hipGetLastError();
 }
 

@@ -34,6 +34,9 @@ for _name, (_res, _args) in PAGED_SIGNATURES.items():
     _fn.restype = _res
     _fn.argtypes = _args
 
+# the handle of a device's current stream, without a Stream object around it where torch has the call for that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
 _append = H.lib.cactus_hip_kv_append_paged_f16_dev
 _read = H.lib.cactus_hip_kv_read_paged_f16_dev
 _attend = H.lib.cactus_hip_attention_paged_f16_dev
@@ -49,63 +52,69 @@ def empty_pages(num_pages, kv_heads, head_dim, page_size=64, device="cuda"):
     return pages(), pages(), scales(), scales()
 
 
+# A decode step calls these functions once per layer with a microsecond or two of work for the GPU, so the checks below read
+# every attribute once, compare device numbers instead of device objects, and put their words together only to raise.
+
 def _need(ok, what):
     if not ok:
         raise ValueError("paged: " + what)
 
 
 def _ints(t, dev, shape, what):
-    if t.dtype != torch.int32 or t.device != dev or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"paged: {what} must be contiguous int32 {list(shape)} on {dev}, got {t.dtype} "
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"paged: {what} must be contiguous int32 {list(shape)} on cuda:{dev}, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(t, dev, shape, what):
     """Address and row stride of fp16 rows [tokens, heads, head_dim]: heads and head_dim contiguous, rows any stride."""
-    if t.dtype != torch.float16 or t.device != dev or t.shape != shape:
-        raise ValueError(f"paged: {what} must be float16 {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
-    _, heads, dim = shape
+    if t.dtype is not torch.float16 or t.get_device() != dev or t.shape != shape:
+        raise ValueError(f"paged: {what} must be float16 {list(shape)} on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+    tokens, heads, dim = shape
     stride, by_head, by_dim = t.stride()
     if by_dim != 1 or (heads > 1 and by_head != dim):
         raise ValueError(f"paged: the heads of a row of {what} must be contiguous, got strides {t.stride()}")
-    return t.data_ptr(), stride if shape[0] > 1 else heads * dim
+    return t.data_ptr(), stride if tokens > 1 else heads * dim
 
 
-def _output(t, dev, shape, what):
+def _output(t, like, dev, shape, what):
     if t is None:
-        return torch.empty(shape, dtype=torch.float16, device=dev)
-    if t.dtype != torch.float16 or t.device != dev or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"paged: {what} must be contiguous float16 {list(shape)} on {dev}")
+        return like.new_empty(shape, dtype=torch.float16)
+    if t.dtype is not torch.float16 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"paged: {what} must be contiguous float16 {list(shape)} on cuda:{dev}")
     return t
 
 
 def _cache(kv, block_tables):
-    """(the C description, device, batch, table width)"""
+    """(the C description, device number, batch, table width)"""
     k, v, ks, vs = kv
-    dev = k.device
-    _need(dev.type == "cuda", f"the cache must be on a GPU, not {dev}")
-    _need(k.dim() == 4 and k.dtype == torch.int8 and k.is_contiguous(), "k pages must be contiguous int8 [pages, kv_heads, "
-          "page_size, head_dim]")
-    _need(v.dtype == torch.int8 and v.shape == k.shape and v.device == dev and v.is_contiguous(),
-          "v pages must be like the k pages")
-    pages, heads, size, dim = k.shape
+    shape, dev = k.shape, k.get_device()
+    if dev < 0:
+        raise ValueError(f"paged: the cache must be on a GPU, not {k.device}")
+    if len(shape) != 4 or k.dtype is not torch.int8 or not k.is_contiguous():
+        raise ValueError("paged: k pages must be contiguous int8 [pages, kv_heads, page_size, head_dim]")
+    if v.shape != shape or v.dtype is not torch.int8 or v.get_device() != dev or not v.is_contiguous():
+        raise ValueError("paged: v pages must be like the k pages")
+    pages, heads, size, dim = shape
     for s in (ks, vs):
-        _need(s.dtype == torch.float32 and s.shape == (pages, heads) and s.device == dev and s.is_contiguous(),
-              "scales must be contiguous float32 [pages, kv_heads] beside the pages")
-    _need(block_tables.dim() == 2, "block_tables must be [batch, width]")
-    _ints(block_tables, dev, block_tables.shape, "block_tables")
-    return (_PagedKv(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, size, heads, dim), dev,
-            block_tables.shape[0], block_tables.shape[1])
+        if s.dtype is not torch.float32 or s.shape != (pages, heads) or s.get_device() != dev or not s.is_contiguous():
+            raise ValueError("paged: scales must be contiguous float32 [pages, kv_heads] beside the pages")
+    table = block_tables.shape
+    _need(len(table) == 2, "block_tables must be [batch, width]")
+    _ints(block_tables, dev, table, "block_tables")
+    return (_PagedKv(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, size, heads, dim), dev, table[0], table[1])
 
 
 def _call(dev, fn, *args):
     """fn on the device's current stream, with the device current while it runs."""
-    if dev.index == torch.cuda.current_device():
-        H._check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            H._check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        H._check(rc)
 
 
 def kv_append(k, v, kv, block_tables, positions, theta, cu_seqlens=None, q=None, q_weight=None, k_weight=None, eps=1e-6,
@@ -127,13 +136,13 @@ def kv_append(k, v, kv, block_tables, positions, theta, cu_seqlens=None, q=None,
         _need(q.dim() == 3, "q must be [tokens, q_heads, head_dim]")
         heads = q.shape[1]
         qp, qst = _rows(q, dev, (tokens, heads, c.head_dim), "q")
-        out_q = _output(out_q, dev, (tokens, heads, c.head_dim), "out_q")
+        out_q = _output(out_q, q, dev, (tokens, heads, c.head_dim), "out_q")
         op = out_q.data_ptr()
     weights = []
     for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None:
-            _need(w.dtype == torch.float16 and w.shape == (c.head_dim,) and w.device == dev and w.is_contiguous(),
-                  f"{what} must be float16 [head_dim]")
+            if w.dtype is not torch.float16 or w.shape != (c.head_dim,) or w.get_device() != dev or not w.is_contiguous():
+                raise ValueError(f"paged: {what} must be float16 [head_dim]")
         weights.append(None if w is None else w.data_ptr())
     _call(dev, _append, C.addressof(c), block_tables.data_ptr(), width, pp, cp, batch, tokens, kp, kst, vp, vst, qp, qst, op,
           heads, weights[0], weights[1], eps, theta)
@@ -145,7 +154,7 @@ def kv_read(kv, block_tables, starts, cu_seqlens, rows, out_k=None, out_v=None):
     c, dev, batch, width = _cache(kv, block_tables)
     sp, cp = _ints(starts, dev, (batch,), "starts"), _ints(cu_seqlens, dev, (batch + 1,), "cu_seqlens")
     shape = (rows, c.kv_heads, c.head_dim)
-    out_k, out_v = _output(out_k, dev, shape, "out_k"), _output(out_v, dev, shape, "out_v")
+    out_k, out_v = _output(out_k, kv[0], dev, shape, "out_k"), _output(out_v, kv[0], dev, shape, "out_v")
     _call(dev, _read, C.addressof(c), block_tables.data_ptr(), width, sp, cp, batch, rows, out_k.data_ptr(), out_v.data_ptr())
     return out_k, out_v
 
@@ -164,10 +173,10 @@ def attention(q, kv, block_tables, context_lens, cu_seqlens=None, max_context=No
     if max_context is None:
         max_context = width * c.page_size
     _need(max_context >= 0 and window >= 0 and sink >= 0, "max_context, window and sink must not be negative")
-    out = _output(out, dev, (tokens, heads, c.head_dim), "out")
+    out = _output(out, q, dev, (tokens, heads, c.head_dim), "out")
     at = C.addressof(c)
     need = _attend_bytes(at, batch, tokens, max_context, heads, window, sink, cp is None)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    work = q.new_empty(need, dtype=torch.uint8) if need else None
     _call(dev, _attend, at, block_tables.data_ptr(), width, xp, cp, batch, tokens, max_context, qp, qst, out.data_ptr(),
           heads, scale, window, sink, work.data_ptr() if need else None, need)
     return out
@@ -176,8 +185,9 @@ def attention(q, kv, block_tables, context_lens, cu_seqlens=None, max_context=No
 def attention_ragged(q, k, v, cu_seqlens, scale=0.0, window=0, sink=0, out=None):
     """Causal FP16 attention of prompts packed by cu_seqlens int32 [batch + 1]: q [tokens, q_heads, head_dim], k / v
     [tokens, kv_heads, head_dim]; window and sink as in attention."""
-    dev = q.device
-    _need(dev.type == "cuda", f"q must be on a GPU, not {dev}")
+    dev = q.get_device()
+    if dev < 0:
+        raise ValueError(f"paged: q must be on a GPU, not {q.device}")
     _need(q.dim() == 3 and k.dim() == 3, "q, k and v must be [tokens, heads, head_dim]")
     _need(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be [batch + 1]")
     _need(window >= 0 and sink >= 0, "window and sink must not be negative")
@@ -188,7 +198,7 @@ def attention_ragged(q, k, v, cu_seqlens, scale=0.0, window=0, sink=0, out=None)
     vp, vst = _rows(v, dev, (tokens, kv_heads, dim), "v")
     batch = cu_seqlens.shape[0] - 1
     cp = _ints(cu_seqlens, dev, (batch + 1,), "cu_seqlens")
-    out = _output(out, dev, (tokens, heads, dim), "out")
+    out = _output(out, q, dev, (tokens, heads, dim), "out")
     _call(dev, _attend_ragged, qp, qst, kp, kst, vp, vst, out.data_ptr(), cp, batch, tokens, heads, kv_heads, dim, scale,
           window, sink)
     return out
