@@ -27,6 +27,12 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TILE_ROWS = 128;
+#ifndef READ_AHEAD
+#define READ_AHEAD 4
+#endif
+#ifndef VALUES_AHEAD
+#define VALUES_AHEAD 4
+#endif
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -151,6 +157,9 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             if (tid < 2 * GROUPS) my_page = page_at(key + 16 * (tid >> 1));
         }
     };
+    // FP16: element offsets of the lane's pieces in a tile (strides are below 2^24)
+    const size_t k_next = 256 / (D / 8) * a.k_stride, v_next = 256 / (D / 8) * a.v_stride;
+    const uint32_t k_lane = tid / (D / 8) * (uint32_t)a.k_stride + tid % (D / 8) * 8, v_lane = tid / (D / 8) * (uint32_t)a.v_stride + tid % (D / 8) * 8;
     const auto fetch = [&](Load& t, int u) {
         const int key = key_of(u);
         if constexpr (PAGED) {
@@ -165,16 +174,34 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             if (tid < 2 * GROUPS)
                 t.scale = my_page < 0 ? -1.0f : fmaxf((tid & 1 ? a.c.vs : a.c.ks)[(size_t)my_page * a.kv_heads + head], 0.0f);
         } else {
+            // a tile's base is the same for all lanes; rows past the last key repeat it
+            const uint16_t* kt = a.k + (size_t)(rows.first + key) * a.k_stride + (size_t)head * D;
+            const uint16_t* vt = a.v + (size_t)(rows.first + key) * a.v_stride + (size_t)head * D;
+            const int most = last - key;
+            if (most >= BK - 1) {
 #pragma unroll
-            for (int i = 0; i < Load::PIECES; i++) {
-                const int p = i * 256 + tid, r = p / (D / 8), d = p % (D / 8) * 8;
-                const size_t from = (size_t)(rows.first + min(key + r, last));   // past the last key: that key again
-                t.k[i] = *reinterpret_cast<const v4i*>(a.k + from * a.k_stride + (size_t)head * D + d);
-                t.v[i] = *reinterpret_cast<const v4i*>(a.v + from * a.v_stride + (size_t)head * D + d);
+                for (int i = 0; i < Load::PIECES; i++) {
+                    t.k[i] = *reinterpret_cast<const v4i*>(kt + i * k_next + k_lane);
+                    t.v[i] = *reinterpret_cast<const v4i*>(vt + i * v_next + v_lane);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < Load::PIECES; i++) {
+                    int p = i * 256 + tid;
+                    asm volatile("" : "+v"(p));          // worked out here, not kept through the loop
+                    const int r = min(p / (D / 8), most), d = p % (D / 8) * 8;
+                    t.k[i] = *reinterpret_cast<const v4i*>(kt + (uint32_t)(r * (int)a.k_stride + d));
+                    t.v[i] = *reinterpret_cast<const v4i*>(vt + (uint32_t)(r * (int)a.v_stride + d));
+                }
             }
         }
     };
-    const auto stash = [&](Load& t, int u, int buf) {
+    // where the lane's pieces go: piece i lies a fixed number of rows below piece 0, at the same place of the swizzle (a chunk pair
+    // of INT8 starts at an even chunk, so its second one is the other of the pair)
+    constexpr int CHUNKS = PAGED ? D / 16 : D / 8, STEP_BYTES = 256 / CHUNKS * ROW;
+    const int to_row = tid / CHUNKS, to_chunk = tid % CHUNKS * (PAGED ? 2 : 1);
+    const uint32_t k_to = to_row * ROW + k_chunk<D>(to_row, to_chunk) * 16, v_to = to_row * ROW + v_chunk<D>(to_row, to_chunk) * 16;
+    const auto stash = [&](auto buf, Load& t, int u) __attribute__((always_inline)) {
         if constexpr (!PAGED) {
             const int key = key_of(u);
             if (key + BK - 1 > pos_of(0) || (a.window && key < last - a.window && key + BK > a.sink)) {
@@ -198,9 +225,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         }
 #pragma unroll
         for (int i = 0; i < Load::PIECES; i++) {
-            const int p = i * 256 + tid;
             if constexpr (PAGED) {
-                const int r = p / (D / 16), c = p % (D / 16) * 2;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
                     v4i x, y;
@@ -214,13 +239,13 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                         y[2 * e] = (int)centred(lo);
                         y[2 * e + 1] = (int)centred(hi);
                     }
-                    *reinterpret_cast<v4i*>(s_k[buf] + r * ROW + k_chunk<D>(r, c + w) * 16) = x;
-                    *reinterpret_cast<v4i*>(s_v[buf] + r * ROW + v_chunk<D>(r, c + w) * 16) = y;
+                    *reinterpret_cast<v4i*>(&s_k[buf][i * STEP_BYTES] + (k_to ^ (16 * w))) = x;
+                    *reinterpret_cast<v4i*>(&s_v[buf][i * STEP_BYTES] + (v_to ^ (16 * w))) = y;
                 }
             } else {
-                const int r = p / (D / 8), c = p % (D / 8);
-                *reinterpret_cast<v4i*>(s_k[buf] + r * ROW + k_chunk<D>(r, c) * 16) = t.k[i];
-                *reinterpret_cast<v4i*>(s_v[buf] + r * ROW + v_chunk<D>(r, c) * 16) = t.v[i];
+                const uint32_t turn = D == 256 && (i & 1) ? 8 * 16 : 0;      // 8 rows on: the other half of K's swizzle
+                *reinterpret_cast<v4i*>(&s_k[buf][i * STEP_BYTES] + (k_to ^ turn)) = t.k[i];
+                *reinterpret_cast<v4i*>(&s_v[buf][i * STEP_BYTES] + v_to) = t.v[i];
             }
         }
         if (PAGED && tid < 2 * GROUPS) s_scale[buf][tid >> 1][tid & 1] = t.scale;
@@ -233,16 +258,22 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
         for (int r = 0; r < 16; r++) o[i][r] = 0.0f;
 
-    // lane addresses: K row n of a 32-key half, chunk 2 s + h; V key 4 h + tq, dims 16 (gi & 1) + 4 tp .. of a 32-dim tile
+    // Lane addresses in a buffer; which buffer, half or group is an immediate offset.  K: row n of a 32-key half, chunk 2 s + h.
+    // V: key 4 h + tq of 16, dims 16 gi + 4 tp .. of a 32-dim tile.
     const int tq = (lane >> 2) & 3, tp = lane & 3, gi = (lane >> 4) & 1;
+    uint32_t k_at[NST], v_at[NDT];
+#pragma unroll
+    for (int i = 0; i < NST; i++) k_at[i] = n * ROW + k_chunk<D>(n, 2 * i + h) * 16;
+#pragma unroll
+    for (int i = 0; i < NDT; i++) v_at[i] = (4 * h + tq) * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
     // the eight keys of group g that a lane holds for its dim of 32-dim tile i
-    const auto value_frag = [&](int buf, int i, int g) __attribute__((always_inline)) {
-        const unsigned char* at = s_v[buf] + (16 * g + 4 * h + tq) * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
+    const auto value_frag = [&](auto buf, int i, int g) __attribute__((always_inline)) {
+        const unsigned char* at = &s_v[buf][16 * g * ROW] + v_at[i];
         const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
         const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * ROW));
         return __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
     };
-    const auto compute = [&](int u, int buf, bool whole) __attribute__((always_inline)) {
+    const auto compute = [&](auto buf, int u, bool whole) __attribute__((always_inline)) {
         const int key = key_of(u);
         v16f s[KT];
 #pragma unroll
@@ -251,10 +282,18 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
 #pragma unroll
             for (int st = 0; st < NST; st++) {
-                const v8h kf = *reinterpret_cast<const v8h*>(s_k[buf] + (32 * t + n) * ROW + k_chunk<D>(n, 2 * st + h) * 16);
+                const v8h kf = *reinterpret_cast<const v8h*>(&s_k[buf][32 * t * ROW] + k_at[st]);
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[st], s[t], 0, 0, 0);
             }
         }
+        // LDS reads run READ_AHEAD ahead of the products that use them
+        __builtin_amdgcn_sched_group_barrier(0x100, READ_AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < KT * NST - READ_AHEAD; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, READ_AHEAD, 0);
         float inv_vs[GROUPS];
         bool live[GROUPS];
         if constexpr (PAGED) {
@@ -269,17 +308,31 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             }
         }
         if (!whole) {
-            // key 32 t + 8 (r / 4) + 4 h + r % 4 of the tile, against this row's last key, first window key and sinks
-            const int to = pos - key - 4 * h, from = a.window ? to - a.window : -BK, sinks = a.sink - key - 4 * h;
+            // key 32 t + 8 (r / 4) + 4 h + r % 4 of the tile, against the row's own key, its first window key and the sinks
+            const int to = pos - key - 4 * h;
+            if (key + BK - 1 > wpos_first) {
 #pragma unroll
-            for (int t = 0; t < KT; t++)
+                for (int t = 0; t < KT; t++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = 32 * t + 8 * (r >> 2) + (r & 3);
-                    bool seen = j <= to && (j >= from || j < sinks);
-                    if constexpr (PAGED) seen = seen && live[2 * t + (r >> 3)];
-                    s[t][r] = seen ? s[t][r] : -INFINITY;
-                }
+                    for (int r = 0; r < 16; r++) s[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) <= to ? s[t][r] : -INFINITY;
+            }
+            if (a.window && key < wpos_last - a.window) {
+                const int from = to - a.window, sinks = a.sink - key - 4 * h;
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int j = 32 * t + 8 * (r >> 2) + (r & 3);
+                        s[t][r] = j >= from || j < sinks ? s[t][r] : -INFINITY;
+                    }
+            }
+            if constexpr (PAGED) {
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++)
+                    if (!live[g])
+#pragma unroll
+                        for (int r = 0; r < 8; r++) s[g >> 1][8 * (g & 1) + r] = -INFINITY;
+            }
         }
         float top = -INFINITY;
 #pragma unroll
@@ -297,7 +350,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[i][r] *= f;
         }
-        v8h p[2 * KT];
+        v8h p[GROUPS];
 #pragma unroll
         for (int g = 0; g < GROUPS; g++) {
             float w[8], sum = 0.0f;
@@ -314,25 +367,38 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 p[g][r] = two[0];
                 p[g][r + 1] = two[1];
             }
-        }
 #pragma unroll
-        for (int i = 0; i < NDT; i++)
-#pragma unroll
-            for (int g = 0; g < GROUPS; g++)
+            for (int i = 0; i < NDT; i++)
                 o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value_frag(buf, i, g), p[g], o[i], 0, 0, 0);
+        }
+        // The first values are read while the first weights are computed; then every product is followed by the reads of one
+        // VALUES_AHEAD further on and a share of the next group's exponentials, which run beside the matrix cores.
+        constexpr int PER_GROUP = 28 + (PAGED ? 1 : 0), SHARE = (PER_GROUP + NDT - 1) / NDT, PRODUCTS = GROUPS * NDT;
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * VALUES_AHEAD, 1);
+        __builtin_amdgcn_sched_group_barrier(0x402, PER_GROUP, 1);
+#pragma unroll
+        for (int i = 0; i < PRODUCTS; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+            if (i < PRODUCTS - VALUES_AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            if (i < PRODUCTS - NDT) __builtin_amdgcn_sched_group_barrier(0x402, SHARE, 1);
+        }
         if constexpr (!PAGED) {
             if (s_odd[buf] == u + 1) {
                 // The values that are not finite are zero in LDS (stash).  Every row that puts weight on such a key is marked:
                 // the output of that dim becomes what adding the value makes of it.
                 uint32_t mine = 0;
 #pragma unroll
-                for (int g = 0; g < GROUPS; g++)
+                for (int g = 0; g < GROUPS; g++) {
+                    v4i bits = __builtin_bit_cast(v4i, p[g]);
+                    asm volatile("" : "+v"(bits));       // not before the branch: without this every tile pays for it
+                    const v8u w = __builtin_bit_cast(v8u, bits);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) mine |= p[g][e] > (_Float16)0.0f || p[g][e] != p[g][e] ? 1u << (8 * g + e) : 0u;
+                    for (int e = 0; e < 8; e++) mine = 2 * mine + (w[e] ? 1u : 0u);       // bit 8 GROUPS - 1 - (8 g + e)
+                }
                 const uint32_t other = __shfl_xor(mine, 32);
 #pragma unroll 1
                 for (int k = 0; k < BK && key + k <= last; k++) {
-                    const int bit = 8 * (k >> 4) + 4 * ((k >> 3) & 1) + (k & 3);
+                    const int bit = 8 * GROUPS - 1 - (8 * (k >> 4) + 4 * ((k >> 3) & 1) + (k & 3));
                     const bool weighed = (((((k >> 2) & 1) == h ? mine : other) >> bit) & 1) != 0;
 #pragma unroll 1
                     for (int d0 = 0; d0 < D; d0 += 64) {
@@ -350,6 +416,8 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     };
 
     if (u0 < u1) {
+        const std::integral_constant<int, 0> zero{};
+        const std::integral_constant<int, 1> one{};
         Load t;
         look_up(u0);
         fetch(t, u0);
@@ -359,9 +427,9 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             for (int i = tid; i < 3 * TILE_ROWS * (D / 32); i += 256) (&s_marks[0][0][0])[i] = 0;
             __syncthreads();
         }
-        stash(t, u0, 0);
+        stash(zero, t, u0);
         __syncthreads();
-        for (int u = u0, buf = 0; u < u1; u++, buf ^= 1) {
+        const auto step = [&](auto buf, auto other, int u) __attribute__((always_inline)) {
             if (u + 1 < u1) {
                 fetch(t, u + 1);
                 look_up(u + 2);
@@ -374,10 +442,14 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                     for (int g = 0; g < GROUPS; g++) whole = whole && s_scale[buf][g][1] >= 0.0f;
                     whole = __builtin_amdgcn_readfirstlane(whole);
                 }
-                compute(u, buf, whole);
+                compute(buf, u, whole);
             }
-            if (u + 1 < u1) stash(t, u + 1, buf ^ 1);
+            if (u + 1 < u1) stash(other, t, u + 1);
             __syncthreads();
+        };
+        for (int u = u0; u < u1; u += 2) {
+            step(zero, one, u);
+            if (u + 1 < u1) step(one, zero, u + 1);
         }
     }
 

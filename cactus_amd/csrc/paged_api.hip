@@ -55,6 +55,7 @@ const char* bad_rows(const void* p, size_t stride, size_t heads, size_t D) {
     if (!p) return "null rows";
     if (!aligned16(p) || stride % 8 != 0) return "rows must be 16-byte aligned, their stride a multiple of 8 elements";
     if (stride < heads * D) return "row stride below heads * head_dim";
+    if (stride >= size_t(1) << 24) return "row stride of 2^24 elements or more";
     return nullptr;
 }
 

@@ -17,7 +17,7 @@
  * Rows (q, k, v, outputs) are packed one sequence behind the other: sequence b owns rows cu_seqlens[b] ..
  * cu_seqlens[b + 1] - 1 of `tokens` (device int32 [batch + 1], not decreasing, starting at 0).  cu_seqlens == NULL: one row
  * per sequence (tokens == batch, a decode step).  Rows behind cu_seqlens[batch] are left as they are.  An input row is
- * half [heads][head_dim]; consecutive rows lie `stride` elements apart (a multiple of 8, at least heads * head_dim: q, k
+ * half [heads][head_dim]; consecutive rows lie `stride` elements apart (a multiple of 8, at least heads * head_dim, below 2^24: q, k
  * and v may be columns of one fused projection); output rows are contiguous.
  *
  * Visibility, in every attention here: position p sees the keys j <= p of its sequence with

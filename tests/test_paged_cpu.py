@@ -90,7 +90,7 @@ def test_refuses_bad_query_rows(call, bad, words):
 
 
 @pytest.mark.parametrize("bad,words", [(dict(positions=None), "positions"), (dict(k=None), "null rows"), (dict(v=None), "null rows"),
-                                       (dict(ks=120), "stride below"), (dict(vs=127), "multiple of 8"), (dict(kw=A + 2), "norm"),
+                                       (dict(ks=120), "stride below"), (dict(ks=1 << 24), "2^24"), (dict(vs=127), "multiple of 8"), (dict(kw=A + 2), "norm"),
                                        (dict(qw=A + 8), "norm"), (dict(theta=-1.0), "theta"), (dict(theta=math.inf), "theta"),
                                        (dict(theta=math.nan), "theta"), (dict(eps=-1e-6), "eps"), (dict(eps=math.nan), "eps")])
 def test_append_refuses(bad, words):
@@ -112,7 +112,7 @@ def test_attention_refuses(bad, words):
 
 @pytest.mark.parametrize("bad,words", [(dict(dim=96), "head_dim"), (dict(cu=None), "cu_seqlens"), (dict(heads=3), "multiple"),
                                        (dict(kv_heads=0), "multiple"), (dict(k=A + 6), "aligned"), (dict(ks=136 - 4), "multiple of 8"),
-                                       (dict(vs=64), "stride below"), (dict(out=None), "null rows"), (dict(scale=-math.inf), "scale"),
+                                       (dict(vs=64), "stride below"), (dict(vs=1 << 30), "2^24"), (dict(out=None), "null rows"), (dict(scale=-math.inf), "scale"),
                                        (dict(window=1 << 40), "window"), (dict(batch=1 << 21), "sequences")])
 def test_ragged_refuses(bad, words):
     assert refused(ragged(**bad), words)
