@@ -79,30 +79,27 @@ struct TileLoad {
     float scale;         // lane 2 g + (0 key, 1 value) of the first wave: the scale of 16-key group g
 };
 
-// Launch order of the slots.  A causal tile's work grows with its position, so late slots go first; when the chip holds the whole
-// launch at two workgroups per CU, the second half goes the other way, so that the two of a CU add up to the same work.
-__device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
-    const int half = (slots + 1) / 2;
-    return slots * kv_heads > 512 || rank < half ? slots - 1 - rank : rank - half;
-}
-
-template <int D, bool PAGED>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+// NG: groups of four waves.  Two groups take every second key tile each and join their (maximum, sum, output) at the end.
+template <int D, bool PAGED, int NG>
+__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int slots) {
     using Load = TileLoad<D, PAGED>;
     constexpr int BK = Load::BK, KT = BK / 32, GROUPS = BK / 16, NST = D / 16, NDT = D / 32, ROW = D * 2;
-    __shared__ __attribute__((aligned(1024))) unsigned char s_k[2][BK * ROW];
-    __shared__ __attribute__((aligned(1024))) unsigned char s_v[2][BK * ROW];
-    __shared__ float s_scale[2][GROUPS][2];
+    __shared__ __attribute__((aligned(1024))) unsigned char s_kv[NG][4][BK * ROW];      // of a group: K, K, V, V
+    __shared__ float s_scales[NG][2][GROUPS][2];
     // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
     // tile, not seen whole by every row, that holds such values; s_marks: +inf, -inf, NaN bits of every row's dims
-    __shared__ int s_odd[2];
+    __shared__ int s_odds[NG][2];
     __shared__ uint32_t s_marks[PAGED ? 1 : 3][PAGED ? 1 : TILE_ROWS][D / 32];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // in the group
+    const int grp = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int n = lane & 31, h = lane >> 5;
-    // kv heads go round first (a head's rows stay in one XCD's L2 when their number divides by 8), heavy slots early
-    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
+    float(*const s_scale)[GROUPS][2] = s_scales[grp];
+    int* const s_odd = s_odds[grp];
+    // kv heads go round first (a head's rows stay in one XCD's L2 when their number divides by 8); a causal tile's work grows with
+    // its position, so late slots go first and the light ones fill the gaps
+    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads;
     const int group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
@@ -141,7 +138,20 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     }
     const float c0 = fabsf(a.scale) * LOG2E;
 
-    const auto key_of = [&](int u) { return (u < plan.sinks ? u : u - plan.sinks + plan.first) * BK; };
+    // tile u of the plan starts at key BK * u (the sinks) or BK * (u + jump)
+    const int jump = plan.first - plan.sinks;
+    const auto key_of = [&](int u) { return (u < plan.sinks ? u : u + jump) * BK; };
+    // What of the plan the wave looks at.  Of the tiles behind the sinks: [seen_lo, seen_hi) hold keys some row sees, [whole_lo,
+    // whole_hi) are seen whole by all its rows.  Of the sinks: all are looked at, the first whole_sinks are seen whole.
+    const auto up = [](int x) { return x <= 0 ? 0 : (x + BK - 1) / BK; };
+    const int seen_hi = wpos_last < 0 ? 0 : wpos_last / BK + 1 - jump;
+    const int whole_hi = wpos_first < 0 ? -jump : (wpos_first + 1) / BK - jump;
+    int seen_lo = plan.sinks, whole_lo = plan.sinks, whole_sinks = 0;
+    if (a.window) {
+        if (a.sink <= plan.first * BK) seen_lo = max(seen_lo, up(wpos_first - a.window - BK + 1) - jump);
+        whole_lo = max(whole_lo, up(wpos_last - a.window) - jump);
+        whole_sinks = min(plan.sinks, a.sink / BK);
+    }
     // page of the 16 keys from `key0`, or -1
     const auto page_at = [&](int key0) { return key0 <= last ? page_of(a.c, b, key0 >> a.c.page_shift) : -1; };
     int pages[Load::PIECES], my_page = -1;                           // of the tile after the next
@@ -196,15 +206,18 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             }
         }
     };
+    // the tiles that every row of the workgroup sees whole
+    const int all_whole_hi = pos_of(0) < 0 ? -jump : (pos_of(0) + 1) / BK - jump;
+    const int all_whole_lo = a.window ? max(plan.sinks, up(last - a.window) - jump) : 0;
     // where the lane's pieces go: piece i lies a fixed number of rows below piece 0, at the same place of the swizzle (a chunk pair
     // of INT8 starts at an even chunk, so its second one is the other of the pair)
     constexpr int CHUNKS = PAGED ? D / 16 : D / 8, STEP_BYTES = 256 / CHUNKS * ROW;
     const int to_row = tid / CHUNKS, to_chunk = tid % CHUNKS * (PAGED ? 2 : 1);
-    const uint32_t k_to = to_row * ROW + k_chunk<D>(to_row, to_chunk) * 16, v_to = to_row * ROW + v_chunk<D>(to_row, to_chunk) * 16;
+    const uint32_t to_base = grp * 4 * BK * ROW + to_row * ROW;
+    const uint32_t k_to = to_base + k_chunk<D>(to_row, to_chunk) * 16, v_to = to_base + v_chunk<D>(to_row, to_chunk) * 16;
     const auto stash = [&](auto buf, Load& t, int u) __attribute__((always_inline)) {
         if constexpr (!PAGED) {
-            const int key = key_of(u);
-            if (key + BK - 1 > pos_of(0) || (a.window && key < last - a.window && key + BK > a.sink)) {
+            if (u >= all_whole_hi || (u < all_whole_lo && u >= whole_sinks)) {
                 uint32_t odd = 0;
 #pragma unroll
                 for (int i = 0; i < Load::PIECES; i++)
@@ -239,13 +252,13 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                         y[2 * e] = (int)centred(lo);
                         y[2 * e + 1] = (int)centred(hi);
                     }
-                    *reinterpret_cast<v4i*>(&s_k[buf][i * STEP_BYTES] + (k_to ^ (16 * w))) = x;
-                    *reinterpret_cast<v4i*>(&s_v[buf][i * STEP_BYTES] + (v_to ^ (16 * w))) = y;
+                    *reinterpret_cast<v4i*>(&s_kv[0][buf][i * STEP_BYTES] + (k_to ^ (16 * w))) = x;
+                    *reinterpret_cast<v4i*>(&s_kv[0][2 + buf][i * STEP_BYTES] + (v_to ^ (16 * w))) = y;
                 }
             } else {
                 const uint32_t turn = D == 256 && (i & 1) ? 8 * 16 : 0;      // 8 rows on: the other half of K's swizzle
-                *reinterpret_cast<v4i*>(&s_k[buf][i * STEP_BYTES] + (k_to ^ turn)) = t.k[i];
-                *reinterpret_cast<v4i*>(&s_v[buf][i * STEP_BYTES] + v_to) = t.v[i];
+                *reinterpret_cast<v4i*>(&s_kv[0][buf][i * STEP_BYTES] + (k_to ^ turn)) = t.k[i];
+                *reinterpret_cast<v4i*>(&s_kv[0][2 + buf][i * STEP_BYTES] + v_to) = t.v[i];
             }
         }
         if (PAGED && tid < 2 * GROUPS) s_scale[buf][tid >> 1][tid & 1] = t.scale;
@@ -263,12 +276,12 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     const int tq = (lane >> 2) & 3, tp = lane & 3, gi = (lane >> 4) & 1;
     uint32_t k_at[NST], v_at[NDT];
 #pragma unroll
-    for (int i = 0; i < NST; i++) k_at[i] = n * ROW + k_chunk<D>(n, 2 * i + h) * 16;
+    for (int i = 0; i < NST; i++) k_at[i] = grp * 4 * BK * ROW + n * ROW + k_chunk<D>(n, 2 * i + h) * 16;
 #pragma unroll
-    for (int i = 0; i < NDT; i++) v_at[i] = (4 * h + tq) * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
+    for (int i = 0; i < NDT; i++) v_at[i] = grp * 4 * BK * ROW + (4 * h + tq) * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
     // the eight keys of group g that a lane holds for its dim of 32-dim tile i
     const auto value_frag = [&](auto buf, int i, int g) __attribute__((always_inline)) {
-        const unsigned char* at = &s_v[buf][16 * g * ROW] + v_at[i];
+        const unsigned char* at = &s_kv[0][2 + buf][16 * g * ROW] + v_at[i];
         const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
         const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * ROW));
         return __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
@@ -277,15 +290,16 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         const int key = key_of(u);
         v16f s[KT];
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
+        for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < NST; st++) {
-                const v8h kf = *reinterpret_cast<const v8h*>(&s_k[buf][32 * t * ROW] + k_at[st]);
+        for (int st = 0; st < NST; st++)
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
+                const v8h kf = *reinterpret_cast<const v8h*>(&s_kv[0][buf][32 * t * ROW] + k_at[st]);
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[st], s[t], 0, 0, 0);
             }
-        }
         // LDS reads run READ_AHEAD ahead of the products that use them
         __builtin_amdgcn_sched_group_barrier(0x100, READ_AHEAD, 0);
 #pragma unroll
@@ -310,13 +324,13 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         if (!whole) {
             // key 32 t + 8 (r / 4) + 4 h + r % 4 of the tile, against the row's own key, its first window key and the sinks
             const int to = pos - key - 4 * h;
-            if (key + BK - 1 > wpos_first) {
+            if (u >= whole_hi) {
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) s[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) <= to ? s[t][r] : -INFINITY;
             }
-            if (a.window && key < wpos_last - a.window) {
+            if (u < whole_lo) {
                 const int from = to - a.window, sinks = a.sink - key - 4 * h;
 #pragma unroll
                 for (int t = 0; t < KT; t++)
@@ -419,24 +433,25 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         const std::integral_constant<int, 0> zero{};
         const std::integral_constant<int, 1> one{};
         Load t;
-        look_up(u0);
-        fetch(t, u0);
-        look_up(u0 + 1);
+        // this group's tiles: first, first + NG, ..; every group takes part in every barrier
+        const int first = u0 + grp;
+        look_up(first);
+        if (first < u1) fetch(t, first);
+        look_up(first + NG);
         if constexpr (!PAGED) {
             if (tid < 2) s_odd[tid] = 0;
-            for (int i = tid; i < 3 * TILE_ROWS * (D / 32); i += 256) (&s_marks[0][0][0])[i] = 0;
+            for (int i = threadIdx.x; i < 3 * TILE_ROWS * (D / 32); i += 256 * NG) (&s_marks[0][0][0])[i] = 0;
             __syncthreads();
         }
-        stash(zero, t, u0);
+        if (first < u1) stash(zero, t, first);
         __syncthreads();
         const auto step = [&](auto buf, auto other, int u) __attribute__((always_inline)) {
-            if (u + 1 < u1) {
-                fetch(t, u + 1);
-                look_up(u + 2);
+            if (u + NG < u1) {
+                fetch(t, u + NG);
+                look_up(u + 2 * NG);
             }
-            const int key = key_of(u);
-            if (key <= wpos_last && (!a.window || key + BK - 1 >= wpos_first - a.window || key < a.sink)) {
-                bool whole = key + BK - 1 <= wpos_first && (!a.window || key >= wpos_last - a.window || key + BK - 1 < a.sink);
+            if (u < seen_hi && (u >= seen_lo || u < plan.sinks) && (NG == 1 || u < u1)) {
+                bool whole = (u >= whole_lo && u < whole_hi) || u < whole_sinks;
                 if constexpr (PAGED) {
 #pragma unroll
                     for (int g = 0; g < GROUPS; g++) whole = whole && s_scale[buf][g][1] >= 0.0f;
@@ -444,16 +459,46 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 }
                 compute(buf, u, whole);
             }
-            if (u + 1 < u1) stash(other, t, u + 1);
+            if (u + NG < u1) stash(other, t, u + NG);
             __syncthreads();
         };
-        for (int u = u0; u < u1; u += 2) {
-            step(zero, one, u);
-            if (u + 1 < u1) step(one, zero, u + 1);
+        for (int u = u0; u < u1; u += 2 * NG) {
+            step(zero, one, u + grp);
+            if (u + NG < u1) step(one, zero, u + NG + grp);
         }
     }
 
     l = pair_sum(l);
+    if constexpr (NG == 2) {
+        // group 1 hands its state over through the tile buffers, 16 bytes a lane and register quad
+        float* state = reinterpret_cast<float*>(&s_kv[0][0][0]) + (wave * NDT * 4 * 64 + lane) * 4;
+        __shared__ float s_ml[TILE_ROWS][2];
+        if (grp == 1) {
+#pragma unroll
+            for (int i = 0; i < NDT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<v4f*>(state + (4 * i + r / 4) * 256) = v4f{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+            if (h == 0) {
+                s_ml[wave * 32 + n][0] = m;
+                s_ml[wave * 32 + n][1] = l;
+            }
+        }
+        __syncthreads();
+        if (grp == 1) return;
+        const float m1 = s_ml[wave * 32 + n][0], l1 = s_ml[wave * 32 + n][1], to = fmaxf(m, m1);
+        const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(m1 - to);
+        m = to;
+        l = l * f0 + l1 * f1;
+#pragma unroll
+        for (int i = 0; i < NDT; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const v4f x = *reinterpret_cast<const v4f*>(state + (4 * i + r / 4) * 256);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[i][r + e] = fmaf(x[e], f1, o[i][r + e] * f0);
+            }
+    }
     if (wave * 32 + n >= R) return;
     const float unit = PAGED ? 512.0f : 1.0f;
     if (splits > 1) {
@@ -500,7 +545,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 template <int D>
 __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int splits, const int slots) {
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = blockIdx.x, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads), group = a.q_heads / a.kv_heads;
+    const int id = blockIdx.x, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads, group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
     const Rows rows = rows_of(a.cu, b, a.tokens);
@@ -530,7 +575,10 @@ __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAtt
 template <int D, bool PAGED>
 hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
     const size_t items = (size_t)s.slots * a.kv_heads;
-    attention_tile_kernel<D, PAGED><<<dim3((unsigned)(items * s.splits)), dim3(256), 0, st>>>(a, s.splits, s.slots);
+    if (D < 256 && s.groups == 2)
+        attention_tile_kernel<D, PAGED, D < 256 ? 2 : 1><<<dim3((unsigned)(items * s.splits)), dim3(512), 0, st>>>(a, s.splits, s.slots);
+    else
+        attention_tile_kernel<D, PAGED, 1><<<dim3((unsigned)(items * s.splits)), dim3(256), 0, st>>>(a, s.splits, s.slots);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || s.splits == 1) return e;
     attention_tile_join_kernel<D><<<dim3((unsigned)items, TILE_ROWS / 4), dim3(256), 0, st>>>(a, s.splits, s.slots);
@@ -541,7 +589,7 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 
 // A tile kernel's launch: a slot per 128 rows of a sequence and kv head, and key splits where that leaves most of the chip idle:
 // as many as fill it twice over, each with at least 512 keys.
-TileShape tile_shape(size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink) {
+TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink) {
     TileShape s;
     const size_t rows = tokens * (q_heads / kv_heads);
     s.slots = (int)(batch == 1 ? (rows + TILE_ROWS - 1) / TILE_ROWS : rows / TILE_ROWS + batch);     // slot_begin
@@ -550,6 +598,7 @@ TileShape tile_shape(size_t batch, size_t tokens, size_t max_context, size_t q_h
     if (window && window + sink + TILE_ROWS < keys) keys = window + sink + TILE_ROWS;
     const size_t most = keys / 512, want = 512 / items;
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
+    s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
     return s;
 }
 size_t tile_record_floats(size_t head_dim) { return TILE_ROWS * (head_dim + 2); }
