@@ -89,7 +89,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     __shared__ float s_scales[NG][2][GROUPS][2];
     // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
     // tile, not seen whole by every row, that holds such values; s_marks: +inf, -inf, NaN bits of every row's dims
-    __shared__ int s_odds[NG][2];
+    __shared__ int s_odds[NG][2], s_marked;
     __shared__ uint32_t s_marks[PAGED ? 1 : 3][PAGED ? 1 : TILE_ROWS][D / 32];
 
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // in the group
@@ -410,6 +410,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                     for (int e = 0; e < 8; e++) mine = 2 * mine + (w[e] ? 1u : 0u);       // bit 8 GROUPS - 1 - (8 g + e)
                 }
                 const uint32_t other = __shfl_xor(mine, 32);
+                s_marked = 1;
 #pragma unroll 1
                 for (int k = 0; k < BK && key + k <= last; k++) {
                     const int bit = 8 * GROUPS - 1 - (8 * (k >> 4) + 4 * ((k >> 3) & 1) + (k & 3));
@@ -440,6 +441,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         look_up(first + NG);
         if constexpr (!PAGED) {
             if (tid < 2) s_odd[tid] = 0;
+            if (threadIdx.x == 0) s_marked = 0;
             for (int i = threadIdx.x; i < 3 * TILE_ROWS * (D / 32); i += 256 * NG) (&s_marks[0][0][0])[i] = 0;
             __syncthreads();
         }
@@ -519,6 +521,20 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             }
     } else {
         const float inv = l > 0.0f || l != l ? unit / l : 0.0f;
+        if constexpr (!PAGED) {
+            if (s_marked) {
+#pragma unroll 1
+                for (int kind = 0; kind < 3; kind++) {
+                    const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+#pragma unroll
+                    for (int i = 0; i < NDT; i++) {
+                        const uint32_t bits = s_marks[kind][wave * 32 + n][i] >> (4 * h);
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[i][r] += (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? add : 0.0f;
+                    }
+                }
+            }
+        }
         uint16_t* out = a.out + ((size_t)token * a.q_heads + qh) * D;
 #pragma unroll
         for (int i = 0; i < NDT; i++)
@@ -526,16 +542,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             for (int r = 0; r < 16; r += 4) {
                 v4h x;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float y = o[i][r + e] * inv;
-                    if constexpr (!PAGED) {
-                        const int at = 2 * r + 4 * h + e;            // of 32-dim tile i
-                        y += (s_marks[0][wave * 32 + n][i] >> at) & 1 ? INFINITY : 0.0f;
-                        y += (s_marks[1][wave * 32 + n][i] >> at) & 1 ? -INFINITY : 0.0f;
-                        y += (s_marks[2][wave * 32 + n][i] >> at) & 1 ? NAN : 0.0f;
-                    }
-                    x[e] = (_Float16)y;
-                }
+                for (int e = 0; e < 4; e++) x[e] = (_Float16)(o[i][r + e] * inv);
                 *reinterpret_cast<v4h*>(out + 32 * i + 2 * r + 4 * h) = x;
             }
     }
