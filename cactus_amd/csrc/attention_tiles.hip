@@ -26,7 +26,10 @@ namespace cactus_hip {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int TILE_ROWS = 128;
+// rows of a wave: 32 (v_mfma_f32_32x32x16_f16), at head_dim 256 16 (v_mfma_f32_16x16x32_f16): 32 rows' output and queries alone
+// are 192 registers there, which leaves one wave per SIMD and every latency in the open
+constexpr int wave_rows(int D) { return D == 256 ? 16 : 32; }
+constexpr int tile_rows(int D) { return 4 * wave_rows(D); }
 #ifndef READ_AHEAD
 #define READ_AHEAD 4
 #endif
@@ -42,6 +45,20 @@ typedef short v8s __attribute__((ext_vector_type(8)));
 typedef unsigned short v8u __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
+template <int RW>
+struct Product;
+template <>
+struct Product<32> {
+    typedef v16f Acc;
+    static __device__ __forceinline__ Acc mul(v8h x, v8h y, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
+};
+template <>
+struct Product<16> {
+    typedef v4f Acc;
+    static __device__ __forceinline__ Acc mul(v8h x, v8h y, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+};
+
+// lanes n, n + RW, .. combine a value
 __device__ __forceinline__ float pair_max(float x) {
     const unsigned u = __float_as_uint(x);
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
@@ -53,11 +70,28 @@ __device__ __forceinline__ float pair_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+__device__ __forceinline__ float half_max(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int RW>
+__device__ __forceinline__ float row_max(float x) { return pair_max(RW == 16 ? half_max(x) : x); }
+template <int RW>
+__device__ __forceinline__ float row_sum(float x) { return pair_sum(RW == 16 ? half_sum(x) : x); }
+
 // 16-byte chunk at which chunk c of a row lies in LDS
 template <int D>
 __device__ __forceinline__ int k_chunk(int row, int c) { return D == 64 ? c ^ ((row >> 1) & 7) : c ^ (row & 15); }
 template <int D>
-__device__ __forceinline__ int v_chunk(int row, int c) { return D == 64 ? c ^ ((row & 2) << 1) : c ^ ((row & 3) << 2); }
+__device__ __forceinline__ int v_chunk(int row, int c) {
+    return D == 64 ? c ^ ((row & 2) << 1) : D == 128 ? c ^ ((row & 3) << 2) : c ^ ((row & 7) << 1);
+}
 
 // four bytes, each ^ 0x80, as halves (b + 128) 2^-24
 __device__ __forceinline__ void offset_halves(uint32_t x, uint32_t& lo, uint32_t& hi) {
@@ -81,10 +115,14 @@ struct TileLoad {
 
 // NG: groups of four waves.  Two groups take every second key tile each and join their (maximum, sum, output) at the end.
 template <int D, bool PAGED, int NG>
-__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2)))
 void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int slots) {
     using Load = TileLoad<D, PAGED>;
-    constexpr int BK = Load::BK, KT = BK / 32, GROUPS = BK / 16, NST = D / 16, NDT = D / 32, ROW = D * 2;
+    // RW rows a wave, lane n + RW h.  An accumulator holds AR values of a lane, quads of four neighbouring keys (dims): key (dim)
+    // QUAD (r / 4) + 4 h + r % 4 of a tile of RW.  Two quads make the eight contracted keys of a lane: FRAGS fragments of FK keys.
+    constexpr int RW = wave_rows(D), LG = 64 / RW, AR = RW * RW / 64, QUAD = 4 * LG, TILE_ROWS = tile_rows(D);
+    constexpr int BK = Load::BK, KT = BK / RW, GROUPS = BK / 16, FK = 8 * LG, FRAGS = BK / FK, NST = D / (8 * LG), NDT = D / RW, ROW = D * 2;
+    typedef typename Product<RW>::Acc Acc;
     __shared__ __attribute__((aligned(1024))) unsigned char s_kv[NG][4][BK * ROW];      // of a group: K, K, V, V
     __shared__ float s_scales[NG][2][GROUPS][2];
     // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
@@ -94,7 +132,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // in the group
     const int grp = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int n = lane & 31, h = lane >> 5;
+    const int n = lane % RW, h = lane / RW;
     float(*const s_scale)[GROUPS][2] = s_scales[grp];
     int* const s_odd = s_odds[grp];
     // kv heads go round first (a head's rows stay in one XCD's L2 when their number divides by 8); a causal tile's work grows with
@@ -110,10 +148,10 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     if (PAGED) context = min(a.contexts[b], a.c.table_width << a.c.page_shift);
     const int pos0 = context - rows.count;                    // position of the sequence's first row
     const auto pos_of = [&](int r) { return pos0 + (tile * TILE_ROWS + r) / group; };
-    const int row = min(wave * 32 + n, R - 1);                       // lanes past the last row repeat it
+    const int row = min(wave * RW + n, R - 1);                       // lanes past the last row repeat it
     const int orow = tile * TILE_ROWS + row, token = rows.first + orow / group, qh = head * group + orow % group;
     const int pos = pos0 + orow / group;
-    const int wpos_first = pos_of(min(wave * 32, R - 1)), wpos_last = pos_of(min(wave * 32 + 31, R - 1));
+    const int wpos_first = pos_of(min(wave * RW, R - 1)), wpos_last = pos_of(min(wave * RW + RW - 1, R - 1));
     const int last = pos_of(R - 1);
     const TilePlan plan = plan_tiles(pos_of(0), last, a.window, a.sink, BK);
     const int per = (plan.tiles + splits - 1) / splits, u0 = split * per, u1 = min(u0 + per, plan.tiles);
@@ -126,7 +164,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int s = 0; s < NST; s++) {
-            v4i x = *reinterpret_cast<const v4i*>(qr + 16 * s + 8 * h);
+            v4i x = *reinterpret_cast<const v4i*>(qr + 8 * LG * s + 8 * h);
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] ^= (int)flip;
             q[s] = __builtin_bit_cast(v8h, x);
@@ -134,7 +172,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
                 for (int e = 0; e < 8; e++) bias += (float)q[s][e];
         }
-        if (PAGED) bias = pair_sum(bias) * -128.0f;
+        if (PAGED) bias = row_sum<RW>(bias) * -128.0f;
     }
     const float c0 = fabsf(a.scale) * LOG2E;
 
@@ -265,40 +303,41 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     };
 
     float m = -1e30f, l = 0.0f;
-    v16f o[NDT];
+    Acc o[NDT];
 #pragma unroll
     for (int i = 0; i < NDT; i++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) o[i][r] = 0.0f;
+        for (int r = 0; r < AR; r++) o[i][r] = 0.0f;
 
-    // Lane addresses in a buffer; which buffer, half or group is an immediate offset.  K: row n of a 32-key half, chunk 2 s + h.
-    // V: key 4 h + tq of 16, dims 16 gi + 4 tp .. of a 32-dim tile.
-    const int tq = (lane >> 2) & 3, tp = lane & 3, gi = (lane >> 4) & 1;
+    // Lane addresses in a buffer; which buffer, tile or fragment is an immediate offset.  K: row n of RW, chunk LG s + h.  V: key
+    // 4 h + tq of QUAD, dims 4 tp .. of 16 (16 gi on where a tile has 32).
+    const int tq = (lane >> 2) & 3, tp = lane & 3, gi = RW == 32 ? (lane >> 4) & 1 : 0;
     uint32_t k_at[NST], v_at[NDT];
 #pragma unroll
-    for (int i = 0; i < NST; i++) k_at[i] = grp * 4 * BK * ROW + n * ROW + k_chunk<D>(n, 2 * i + h) * 16;
+    for (int i = 0; i < NST; i++) k_at[i] = grp * 4 * BK * ROW + n * ROW + k_chunk<D>(n, LG * i + h) * 16;
 #pragma unroll
-    for (int i = 0; i < NDT; i++) v_at[i] = grp * 4 * BK * ROW + (4 * h + tq) * ROW + v_chunk<D>(tq, 4 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
-    // the eight keys of group g that a lane holds for its dim of 32-dim tile i
-    const auto value_frag = [&](auto buf, int i, int g) __attribute__((always_inline)) {
-        const unsigned char* at = &s_kv[0][2 + buf][16 * g * ROW] + v_at[i];
+    for (int i = 0; i < NDT; i++)
+        v_at[i] = grp * 4 * BK * ROW + (4 * h + tq) * ROW + v_chunk<D>(4 * h + tq, RW / 8 * i + 2 * gi + (tp >> 1)) * 16 + (tp & 1) * 8;
+    // the eight keys of fragment f that a lane holds for its dim of dim tile i
+    const auto value_frag = [&](auto buf, int i, int f) __attribute__((always_inline)) {
+        const unsigned char* at = &s_kv[0][2 + buf][FK * f * ROW] + v_at[i];
         const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
-        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * ROW));
+        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + QUAD * ROW));
         return __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
     };
     const auto compute = [&](auto buf, int u, bool whole) __attribute__((always_inline)) {
         const int key = key_of(u);
-        v16f s[KT];
+        Acc s[KT];
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[t][r] = 0.0f;
+            for (int r = 0; r < AR; r++) s[t][r] = 0.0f;
 #pragma unroll
         for (int st = 0; st < NST; st++)
 #pragma unroll
             for (int t = 0; t < KT; t++) {
-                const v8h kf = *reinterpret_cast<const v8h*>(&s_kv[0][buf][32 * t * ROW] + k_at[st]);
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[st], s[t], 0, 0, 0);
+                const v8h kf = *reinterpret_cast<const v8h*>(&s_kv[0][buf][RW * t * ROW] + k_at[st]);
+                s[t] = Product<RW>::mul(kf, q[st], s[t]);
             }
         // LDS reads run READ_AHEAD ahead of the products that use them
         __builtin_amdgcn_sched_group_barrier(0x100, READ_AHEAD, 0);
@@ -308,52 +347,58 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, READ_AHEAD, 0);
+        const auto group_of = [](int t, int r) { return (RW * t + QUAD * (r >> 2)) / 16; };      // 16-key group of a score
         float inv_vs[GROUPS];
         bool live[GROUPS];
         if constexpr (PAGED) {
+            float up[GROUPS], add[GROUPS];
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
                 const float ks = s_scale[buf][g][0], v0 = s_scale[buf][g][1], vs = fmaxf(v0, 1e-20f);
                 live[g] = v0 >= 0.0f;
-                const float c = c0 * ks, up = c * 16777216.0f, add = fmaf(c, bias, __log2f(vs));
+                const float c = c0 * ks;
+                up[g] = c * 16777216.0f;
+                add[g] = fmaf(c, bias, __log2f(vs));
                 inv_vs[g] = 1.0f / vs;
-#pragma unroll
-                for (int r = 0; r < 8; r++) s[g >> 1][8 * (g & 1) + r] = fmaf(s[g >> 1][8 * (g & 1) + r], up, add);
             }
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < AR; r++) s[t][r] = fmaf(s[t][r], up[group_of(t, r)], add[group_of(t, r)]);
         }
         if (!whole) {
-            // key 32 t + 8 (r / 4) + 4 h + r % 4 of the tile, against the row's own key, its first window key and the sinks
+            // a score's key against the row's own key, its first window key and the sinks
             const int to = pos - key - 4 * h;
             if (u >= whole_hi) {
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) <= to ? s[t][r] : -INFINITY;
+                    for (int r = 0; r < AR; r++) s[t][r] = RW * t + QUAD * (r >> 2) + (r & 3) <= to ? s[t][r] : -INFINITY;
             }
             if (u < whole_lo) {
                 const int from = to - a.window, sinks = a.sink - key - 4 * h;
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int j = 32 * t + 8 * (r >> 2) + (r & 3);
+                    for (int r = 0; r < AR; r++) {
+                        const int j = RW * t + QUAD * (r >> 2) + (r & 3);
                         s[t][r] = j >= from || j < sinks ? s[t][r] : -INFINITY;
                     }
             }
             if constexpr (PAGED) {
 #pragma unroll
-                for (int g = 0; g < GROUPS; g++)
-                    if (!live[g])
+                for (int t = 0; t < KT; t++)
 #pragma unroll
-                        for (int r = 0; r < 8; r++) s[g >> 1][8 * (g & 1) + r] = -INFINITY;
+                    for (int r = 0; r < AR; r++)
+                        if (!live[group_of(t, r)]) s[t][r] = -INFINITY;
             }
         }
         float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(s[t][r], s[t][r + 1]), top);
-        top = pair_max(top);
+            for (int r = 0; r < AR; r += 2) top = fmaxf(fmaxf(s[t][r], s[t][r + 1]), top);
+        top = row_max<RW>(top);
         if (!PAGED) top *= c0;
         if (__any(top > m + 8.0f)) {
             const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
@@ -362,34 +407,34 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
             for (int i = 0; i < NDT; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) o[i][r] *= f;
+                for (int r = 0; r < AR; r++) o[i][r] *= f;
         }
-        v8h p[GROUPS];
+        v8h p[FRAGS];
 #pragma unroll
-        for (int g = 0; g < GROUPS; g++) {
-            float w[8], sum = 0.0f;
+        for (int f = 0; f < FRAGS; f++) {
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const float x = s[g >> 1][8 * (g & 1) + r];
-                w[r] = __builtin_amdgcn_exp2f(PAGED ? x - m : fmaf(x, c0, -m));
-                sum += w[r];
+            for (int half = 0; half < 2; half++) {
+                const int quad = 2 * f + half, t = quad / (AR / 4), r0 = quad % (AR / 4) * 4;
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(PAGED ? s[t][r0 + e] - m : fmaf(s[t][r0 + e], c0, -m));
+                const float sum = (w[0] + w[1]) + (w[2] + w[3]);
+                l = PAGED ? fmaf(sum, inv_vs[group_of(t, r0)], l) : l + sum;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const v2h two = __builtin_convertvector(v2f{w[e], w[e + 1]}, v2h);
+                    p[f][4 * half + e] = two[0];
+                    p[f][4 * half + e + 1] = two[1];
+                }
             }
-            l = PAGED ? fmaf(sum, inv_vs[g], l) : l + sum;
 #pragma unroll
-            for (int r = 0; r < 8; r += 2) {
-                const v2h two = __builtin_convertvector(v2f{w[r], w[r + 1]}, v2h);
-                p[g][r] = two[0];
-                p[g][r + 1] = two[1];
-            }
-#pragma unroll
-            for (int i = 0; i < NDT; i++)
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value_frag(buf, i, g), p[g], o[i], 0, 0, 0);
+            for (int i = 0; i < NDT; i++) o[i] = Product<RW>::mul(value_frag(buf, i, f), p[f], o[i]);
         }
         // The first values are read while the first weights are computed; then every product is followed by the reads of one
-        // VALUES_AHEAD further on and a share of the next group's exponentials, which run beside the matrix cores.
-        constexpr int PER_GROUP = 28 + (PAGED ? 1 : 0), SHARE = (PER_GROUP + NDT - 1) / NDT, PRODUCTS = GROUPS * NDT;
+        // VALUES_AHEAD further on and a share of the next fragment's exponentials, which run beside the matrix cores.
+        constexpr int PER_FRAG = 28, SHARE = (PER_FRAG + NDT - 1) / NDT, PRODUCTS = FRAGS * NDT;
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * VALUES_AHEAD, 1);
-        __builtin_amdgcn_sched_group_barrier(0x402, PER_GROUP, 1);
+        __builtin_amdgcn_sched_group_barrier(0x402, PER_FRAG, 1);
 #pragma unroll
         for (int i = 0; i < PRODUCTS; i++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
@@ -402,19 +447,18 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 // the output of that dim becomes what adding the value makes of it.
                 uint32_t mine = 0;
 #pragma unroll
-                for (int g = 0; g < GROUPS; g++) {
-                    v4i bits = __builtin_bit_cast(v4i, p[g]);
+                for (int f = 0; f < FRAGS; f++) {
+                    v4i bits = __builtin_bit_cast(v4i, p[f]);
                     asm volatile("" : "+v"(bits));       // not before the branch: without this every tile pays for it
                     const v8u w = __builtin_bit_cast(v8u, bits);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) mine = 2 * mine + (w[e] ? 1u : 0u);       // bit 8 GROUPS - 1 - (8 g + e)
+                    for (int e = 0; e < 8; e++) mine = 2 * mine + (w[e] ? 1u : 0u);       // bit 8 FRAGS - 1 - (8 f + e)
                 }
-                const uint32_t other = __shfl_xor(mine, 32);
                 s_marked = 1;
 #pragma unroll 1
                 for (int k = 0; k < BK && key + k <= last; k++) {
-                    const int bit = 8 * GROUPS - 1 - (8 * (k >> 4) + 4 * ((k >> 3) & 1) + (k & 3));
-                    const bool weighed = (((((k >> 2) & 1) == h ? mine : other) >> bit) & 1) != 0;
+                    const int in = k % FK, bit = 8 * FRAGS - 1 - (8 * (k / FK) + 4 * (in / QUAD) + (k & 3));
+                    const bool weighed = ((__shfl(mine, n + RW * (in % QUAD / 4)) >> bit) & 1) != 0;
 #pragma unroll 1
                     for (int d0 = 0; d0 < D; d0 += 64) {
                         const uint32_t x = a.v[(size_t)(rows.first + key + k) * a.v_stride + (size_t)head * D + d0 + lane];
@@ -422,7 +466,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                             const int at = __builtin_ctzll(odd), d = d0 + at;
                             const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)x, at);
                             const int kind = y == 0x7c00u ? 0 : y == 0xfc00u ? 1 : 2;
-                            if (weighed) atomicOr(&s_marks[kind][wave * 32 + n][d >> 5], 1u << (d & 31));
+                            if (weighed) atomicOr(&s_marks[kind][wave * RW + n][d >> 5], 1u << (d & 31));
                         }
                     }
                 }
@@ -470,38 +514,38 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         }
     }
 
-    l = pair_sum(l);
+    l = row_sum<RW>(l);
     if constexpr (NG == 2) {
         // group 1 hands its state over through the tile buffers, 16 bytes a lane and register quad
-        float* state = reinterpret_cast<float*>(&s_kv[0][0][0]) + (wave * NDT * 4 * 64 + lane) * 4;
+        float* state = reinterpret_cast<float*>(&s_kv[0][0][0]) + (wave * NDT * (AR / 4) * 64 + lane) * 4;
         __shared__ float s_ml[TILE_ROWS][2];
         if (grp == 1) {
 #pragma unroll
             for (int i = 0; i < NDT; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    *reinterpret_cast<v4f*>(state + (4 * i + r / 4) * 256) = v4f{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+                for (int r = 0; r < AR; r += 4)
+                    *reinterpret_cast<v4f*>(state + (AR * i + r) * 64) = v4f{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
             if (h == 0) {
-                s_ml[wave * 32 + n][0] = m;
-                s_ml[wave * 32 + n][1] = l;
+                s_ml[wave * RW + n][0] = m;
+                s_ml[wave * RW + n][1] = l;
             }
         }
         __syncthreads();
         if (grp == 1) return;
-        const float m1 = s_ml[wave * 32 + n][0], l1 = s_ml[wave * 32 + n][1], to = fmaxf(m, m1);
+        const float m1 = s_ml[wave * RW + n][0], l1 = s_ml[wave * RW + n][1], to = fmaxf(m, m1);
         const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(m1 - to);
         m = to;
         l = l * f0 + l1 * f1;
 #pragma unroll
         for (int i = 0; i < NDT; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const v4f x = *reinterpret_cast<const v4f*>(state + (4 * i + r / 4) * 256);
+            for (int r = 0; r < AR; r += 4) {
+                const v4f x = *reinterpret_cast<const v4f*>(state + (AR * i + r) * 64);
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[i][r + e] = fmaf(x[e], f1, o[i][r + e] * f0);
             }
     }
-    if (wave * 32 + n >= R) return;
+    if (wave * RW + n >= R) return;
     const float unit = PAGED ? 512.0f : 1.0f;
     if (splits > 1) {
         float* record = a.work + (size_t)blockIdx.x * TILE_ROWS * (D + 2);
@@ -509,15 +553,15 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             record[2 * row] = m;
             record[2 * row + 1] = l;
         }
-        float* out = record + 2 * TILE_ROWS + (size_t)row * D;
+        float* out = record + 2 * TILE_ROWS + (size_t)row * D + 4 * h;
 #pragma unroll
         for (int i = 0; i < NDT; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
+            for (int r = 0; r < AR; r += 4) {
                 v4f x;
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[e] = o[i][r + e] * unit;
-                *reinterpret_cast<v4f*>(out + 32 * i + 2 * r + 4 * h) = x;
+                *reinterpret_cast<v4f*>(out + RW * i + QUAD * (r >> 2)) = x;
             }
     } else {
         const float inv = l > 0.0f || l != l ? unit / l : 0.0f;
@@ -527,23 +571,24 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 for (int kind = 0; kind < 3; kind++) {
                     const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
 #pragma unroll
-                    for (int i = 0; i < NDT; i++) {
-                        const uint32_t bits = s_marks[kind][wave * 32 + n][i] >> (4 * h);
+                    for (int i = 0; i < NDT; i++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) o[i][r] += (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? add : 0.0f;
-                    }
+                        for (int r = 0; r < AR; r++) {
+                            const int d = RW * i + QUAD * (r >> 2) + (r & 3);      // and 4 h, which stays inside the word
+                            o[i][r] += (s_marks[kind][wave * RW + n][d >> 5] >> ((d & 31) + 4 * h)) & 1 ? add : 0.0f;
+                        }
                 }
             }
         }
-        uint16_t* out = a.out + ((size_t)token * a.q_heads + qh) * D;
+        uint16_t* out = a.out + ((size_t)token * a.q_heads + qh) * D + 4 * h;
 #pragma unroll
         for (int i = 0; i < NDT; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
+            for (int r = 0; r < AR; r += 4) {
                 v4h x;
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[e] = (_Float16)(o[i][r + e] * inv);
-                *reinterpret_cast<v4h*>(out + 32 * i + 2 * r + 4 * h) = x;
+                *reinterpret_cast<v4h*>(out + RW * i + QUAD * (r >> 2)) = x;
             }
     }
 }
@@ -551,6 +596,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 // joins the splits of a tile's rows: a wave per row, lanes = dims
 template <int D>
 __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int splits, const int slots) {
+    constexpr int TILE_ROWS = tile_rows(D);
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = blockIdx.x, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads, group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
@@ -588,27 +634,28 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
         attention_tile_kernel<D, PAGED, 1><<<dim3((unsigned)(items * s.splits)), dim3(256), 0, st>>>(a, s.splits, s.slots);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || s.splits == 1) return e;
-    attention_tile_join_kernel<D><<<dim3((unsigned)items, TILE_ROWS / 4), dim3(256), 0, st>>>(a, s.splits, s.slots);
+    attention_tile_join_kernel<D><<<dim3((unsigned)items, tile_rows(D) / 4), dim3(256), 0, st>>>(a, s.splits, s.slots);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// A tile kernel's launch: a slot per 128 rows of a sequence and kv head, and key splits where that leaves most of the chip idle:
-// as many as fill it twice over, each with at least 512 keys.
-TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink) {
+// A tile kernel's launch: a slot per tile of a sequence's rows and kv head, and key splits where that leaves most of the chip
+// idle: as many as fill it twice over, each with at least 512 keys.
+TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
+                     size_t window, size_t sink) {
     TileShape s;
-    const size_t rows = tokens * (q_heads / kv_heads);
-    s.slots = (int)(batch == 1 ? (rows + TILE_ROWS - 1) / TILE_ROWS : rows / TILE_ROWS + batch);     // slot_begin
+    const size_t rows = tokens * (q_heads / kv_heads), size = tile_rows((int)head_dim);
+    s.slots = (int)(batch == 1 ? (rows + size - 1) / size : rows / size + batch);     // slot_begin
     const size_t items = (size_t)s.slots * kv_heads;
     size_t keys = max_context;
-    if (window && window + sink + TILE_ROWS < keys) keys = window + sink + TILE_ROWS;
+    if (window && window + sink + size < keys) keys = window + sink + size;
     const size_t most = keys / 512, want = 512 / items;
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
     s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
     return s;
 }
-size_t tile_record_floats(size_t head_dim) { return TILE_ROWS * (head_dim + 2); }
+size_t tile_record_floats(size_t head_dim) { return tile_rows((int)head_dim) * (head_dim + 2); }
 
 hipError_t launch_attention_tiles(int D, bool paged, const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
     if (paged) return D == 64 ? launch<64, true>(a, s, st) : D == 128 ? launch<128, true>(a, s, st) : launch<256, true>(a, s, st);
