@@ -113,6 +113,18 @@ struct TileLoad {
     float scale;         // lane 2 g + (0 key, 1 value) of the first wave: the scale of 16-key group g
 };
 
+// The slot of a workgroup.  A causal tile's work grows with its position, so late slots go first and the light ones fill the gaps.
+// Workgroups go round the 8 XCDs, and so do the kv heads: with 8 of them a head's rows stay in one L2.  With fewer, ranks are
+// dealt to the XCDs that share a head 8 neighbours at a time, because neighbours read the same keys (windowed prompts of one
+// kv head 121 -> 101 us; 4 to 32 neighbours measure the same).
+__device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
+    constexpr int NEIGHBOURS = 8;
+    const int share = kv_heads % 8 == 0 ? 1 : kv_heads % 4 == 0 ? 2 : kv_heads % 2 == 0 ? 4 : 8, block = share * NEIGHBOURS;
+    const int base = rank / block * block, in = rank - base;
+    if (share > 1 && base + block <= slots) rank = base + in % share * NEIGHBOURS + in / share;
+    return slots - 1 - rank;
+}
+
 // NG: groups of four waves.  Two groups take every second key tile each and join their (maximum, sum, output) at the end.
 template <int D, bool PAGED, int NG>
 __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2)))
@@ -135,9 +147,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     const int n = lane % RW, h = lane / RW;
     float(*const s_scale)[GROUPS][2] = s_scales[grp];
     int* const s_odd = s_odds[grp];
-    // kv heads go round first (a head's rows stay in one XCD's L2 when their number divides by 8); a causal tile's work grows with
-    // its position, so late slots go first and the light ones fill the gaps
-    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads;
+    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
     const int group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
@@ -598,7 +608,7 @@ template <int D>
 __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int splits, const int slots) {
     constexpr int TILE_ROWS = tile_rows(D);
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = blockIdx.x, head = id % a.kv_heads, slot = slots - 1 - id / a.kv_heads, group = a.q_heads / a.kv_heads;
+    const int id = blockIdx.x, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads), group = a.q_heads / a.kv_heads;
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
     const Rows rows = rows_of(a.cu, b, a.tokens);
