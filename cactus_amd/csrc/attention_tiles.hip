@@ -110,7 +110,8 @@ struct TileLoad {
     static constexpr int BK = D == 256 ? 32 : 64;
     static constexpr int PIECES = BK * D * (PAGED ? 1 : 2) / 16 / 256;      // per thread and operand
     v4i k[PIECES], v[PIECES];
-    float scale;         // lane 2 g + (0 key, 1 value) of the first wave: the scale of 16-key group g
+    float scale;         // lane 2 g + (0 key, 1 value): the scale of 16-key group g, and its page
+    int page;
 };
 
 // The slot of a workgroup.  A causal tile's work grows with its position, so late slots go first and the light ones fill the gaps.
@@ -202,7 +203,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     }
     // page of the 16 keys from `key0`, or -1
     const auto page_at = [&](int key0) { return key0 <= last ? page_of(a.c, b, key0 >> a.c.page_shift) : -1; };
-    int pages[Load::PIECES], my_page = -1;                           // of the tile after the next
+    int pages[Load::PIECES] = {}, my_page = -1;                         // of the tile after the next
     const auto look_up = [&](int u) {
         if constexpr (PAGED) {
             if (u >= u1) return;
@@ -212,12 +213,12 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 const int r = (i * 256 + wave * 64) / (D / 16);      // the wave's rows lie in one 16-key group
                 pages[i] = page_at(key + (r & ~15));
             }
-            if (tid < 2 * GROUPS) my_page = page_at(key + 16 * (tid >> 1));
+            my_page = page_at(key + 16 * (tid % (2 * GROUPS) >> 1));
         }
     };
     // FP16: element offsets of the lane's pieces in a tile (strides are below 2^24)
-    const size_t k_next = 256 / (D / 8) * a.k_stride, v_next = 256 / (D / 8) * a.v_stride;
-    const uint32_t k_lane = tid / (D / 8) * (uint32_t)a.k_stride + tid % (D / 8) * 8, v_lane = tid / (D / 8) * (uint32_t)a.v_stride + tid % (D / 8) * 8;
+    const uint32_t k_next = 512 / (D / 8) * a.k_stride, v_next = 512 / (D / 8) * a.v_stride;
+    const uint32_t k_lane = 2 * (tid / (D / 8) * (uint32_t)a.k_stride + tid % (D / 8) * 8), v_lane = 2 * (tid / (D / 8) * (uint32_t)a.v_stride + tid % (D / 8) * 8);
     const auto fetch = [&](Load& t, int u) {
         const int key = key_of(u);
         if constexpr (PAGED) {
@@ -229,29 +230,19 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 t.k[i] = *reinterpret_cast<const v4i*>(a.c.k + from);
                 t.v[i] = *reinterpret_cast<const v4i*>(a.c.v + from);
             }
-            if (tid < 2 * GROUPS)
-                t.scale = my_page < 0 ? -1.0f : fmaxf((tid & 1 ? a.c.vs : a.c.ks)[(size_t)my_page * a.kv_heads + head], 0.0f);
+            t.scale = (tid & 1 ? a.c.vs : a.c.ks)[(size_t)max(my_page, 0) * a.kv_heads + head];
+            t.page = my_page;
         } else {
-            // a tile's base is the same for all lanes; rows past the last key repeat it
-            const uint16_t* kt = a.k + (size_t)(rows.first + key) * a.k_stride + (size_t)head * D;
-            const uint16_t* vt = a.v + (size_t)(rows.first + key) * a.v_stride + (size_t)head * D;
-            const int most = last - key;
-            if (most >= BK - 1) {
+            // a tile's base is the same for all lanes; rows past the last key read as zero
+            const int most = u < u1 ? min(last - key, BK - 1) : -1;
+            const auto kb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.k) + (size_t)(rows.first + key) * a.k_stride + (size_t)head * D, 0, most < 0 ? 0 : 2 * (most * (int)a.k_stride + D), 0x00027000);
+            const auto vb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.v) + (size_t)(rows.first + key) * a.v_stride + (size_t)head * D, 0, most < 0 ? 0 : 2 * (most * (int)a.v_stride + D), 0x00027000);
 #pragma unroll
-                for (int i = 0; i < Load::PIECES; i++) {
-                    t.k[i] = *reinterpret_cast<const v4i*>(kt + i * k_next + k_lane);
-                    t.v[i] = *reinterpret_cast<const v4i*>(vt + i * v_next + v_lane);
-                }
-            } else {
+            for (int i = 0; i < Load::PIECES; i++)
+                t.k[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, k_lane + i * k_next, 0, 0));
 #pragma unroll
-                for (int i = 0; i < Load::PIECES; i++) {
-                    int p = i * 256 + tid;
-                    asm volatile("" : "+v"(p));          // worked out here, not kept through the loop
-                    const int r = min(p / (D / 8), most), d = p % (D / 8) * 8;
-                    t.k[i] = *reinterpret_cast<const v4i*>(kt + (uint32_t)(r * (int)a.k_stride + d));
-                    t.v[i] = *reinterpret_cast<const v4i*>(vt + (uint32_t)(r * (int)a.v_stride + d));
-                }
-            }
+            for (int i = 0; i < Load::PIECES; i++)
+                t.v[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vb, v_lane + i * v_next, 0, 0));
         }
     };
     // the tiles that every row of the workgroup sees whole
@@ -309,7 +300,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 *reinterpret_cast<v4i*>(&s_kv[0][2 + buf][i * STEP_BYTES] + v_to) = t.v[i];
             }
         }
-        if (PAGED && tid < 2 * GROUPS) s_scale[buf][tid >> 1][tid & 1] = t.scale;
+        if (PAGED && tid < 2 * GROUPS) s_scale[buf][tid >> 1][tid & 1] = t.page < 0 ? -1.0f : fmaxf(t.scale, 0.0f);
     };
 
     float m = -1e30f, l = 0.0f;
@@ -335,13 +326,14 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + QUAD * ROW));
         return __builtin_bit_cast(v8h, v8s{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
     };
-    const auto compute = [&](auto buf, int u, bool whole) __attribute__((always_inline)) {
+    const auto compute = [&](auto buf, Load& t, int u, bool whole) __attribute__((always_inline)) {
         const int key = key_of(u);
+        fetch(t, u + NG);
         Acc s[KT];
 #pragma unroll
-        for (int t = 0; t < KT; t++)
+        for (int j = 0; j < KT; j++)
 #pragma unroll
-            for (int r = 0; r < AR; r++) s[t][r] = 0.0f;
+            for (int r = 0; r < AR; r++) s[j][r] = 0.0f;
 #pragma unroll
         for (int st = 0; st < NST; st++)
 #pragma unroll
@@ -355,6 +347,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         for (int i = 0; i < KT * NST - READ_AHEAD; i++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (i < 2 * Load::PIECES) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, READ_AHEAD, 0);
         const auto group_of = [](int t, int r) { return (RW * t + QUAD * (r >> 2)) / 16; };      // 16-key group of a score
@@ -502,19 +495,18 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         if (first < u1) stash(zero, t, first);
         __syncthreads();
         const auto step = [&](auto buf, auto other, int u) __attribute__((always_inline)) {
-            if (u + NG < u1) {
-                fetch(t, u + NG);
-                look_up(u + 2 * NG);
-            }
-            if (u < seen_hi && (u >= seen_lo || u < plan.sinks) && (NG == 1 || u < u1)) {
+            const bool seen = u < seen_hi && (u >= seen_lo || u < plan.sinks) && (NG == 1 || u < u1);
+            if (!seen && u + NG < u1) fetch(t, u + NG);
+            if (seen) {
                 bool whole = (u >= whole_lo && u < whole_hi) || u < whole_sinks;
                 if constexpr (PAGED) {
 #pragma unroll
                     for (int g = 0; g < GROUPS; g++) whole = whole && s_scale[buf][g][1] >= 0.0f;
                     whole = __builtin_amdgcn_readfirstlane(whole);
                 }
-                compute(buf, u, whole);
+                compute(buf, t, u, whole);
             }
+            look_up(u + 2 * NG);
             if (u + NG < u1) stash(other, t, u + NG);
             __syncthreads();
         };
