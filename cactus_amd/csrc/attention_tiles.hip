@@ -1,20 +1,29 @@
 // Attention of many query rows (include/cactus_hip_paged.h): packed FP16 prompts, and prompt chunks over the paged INT8
-// cache.  Bound: matrix cores and the softmax's vector instructions, which share a SIMD's issue port.
+// cache.  Bound: the matrix cores, the softmax's vector instructions and the LDS reads together, none of them alone: of the
+// 4800 cycles that two waves of a SIMD take for a key tile each (D = 128) the matrix cores work 2050.
 //
-// A workgroup is four waves on 128 consecutive rows of one (sequence, kv head); a row is (token, query head of the group), so a
-// key tile in LDS serves all query heads of its kv head.  A wave owns 32 rows and computes everything transposed, a lane
-// owning a row (lane % 32):
+// A workgroup is four waves on 128 consecutive rows (64 at head_dim 256) of one (sequence, kv head); a row is (token, query head
+// of the group), so a key tile in LDS serves all query heads of its kv head.  A wave owns 32 rows (16) and computes everything
+// transposed, a lane owning a row (lane % 32):
 //   S^T = K Q^T   v_mfma_f32_32x32x16_f16, K rows from LDS, the wave's Q in registers for the whole kernel
 //   O^T = V^T P^T V^T through the transposing LDS read (ds_read_b64_tr_b16); P is the lane's own scores, in the key order the
 //                 first product left them in (the contraction order is free)
 // so the softmax's maximum and sum are in-lane work plus one exchange with lane ^ 32, and weights never move.  The rest is the
 // online softmax in base 2; (l, O) move to a new maximum only when it has grown by more than 2^8.
-// Key tiles (64 keys, 32 at head_dim 256) are double-buffered: the next one is loaded into registers before the current one is
-// computed and stored to the other buffer behind it, one barrier per tile.  16-byte chunks of a row are swizzled so that neither
-// the row reads of K (16 rows, one chunk) nor the transposed reads of V (4 rows, 4 chunks) meet on a bank.
+// Key tiles (64 keys, 32 at head_dim 256) are double-buffered: the next one's loads go out between the products of the scores (a
+// burst of them holds every wave up) and it is stored to the other buffer behind the output's products, one barrier per tile.
+// Loads past a sequence's last row are cut off by the buffer's length and give zeros, so no tile needs a branch.  16-byte chunks
+// of a row are swizzled so that neither the row reads of K (16 rows, one chunk) nor the transposed reads of V (4 rows, 4 chunks)
+// meet on a bank.
 // INT8 pages become halves on the way into LDS: keys as the subnormal (b + 128) 2^-24 (one v_perm per two; the offset leaves
 // with the score's fma), values as b 2^-9.  Page scales enter as in attention_paged.hip.
 // Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count); everything else is fp32.
+//
+// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 819 TFLOP/s (a large FP16 matrix product reaches
+// 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 91 us, 466.  24 prompts of 17 to 300 tokens,
+// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 53.5 us, 10 of them the join's.
+// Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
+// turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
 
 #include <math.h>
@@ -30,12 +39,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 // are 192 registers there, which leaves one wave per SIMD and every latency in the open
 constexpr int wave_rows(int D) { return D == 256 ? 16 : 32; }
 constexpr int tile_rows(int D) { return 4 * wave_rows(D); }
-#ifndef READ_AHEAD
-#define READ_AHEAD 4
-#endif
-#ifndef VALUES_AHEAD
-#define VALUES_AHEAD 4
-#endif
+// products that the LDS reads run ahead of (3 measures the same, 6 up to 1% slower, 2 up to 4%)
+constexpr int READ_AHEAD = 4;
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -117,7 +122,7 @@ struct TileLoad {
 // The slot of a workgroup.  A causal tile's work grows with its position, so late slots go first and the light ones fill the gaps.
 // Workgroups go round the 8 XCDs, and so do the kv heads: with 8 of them a head's rows stay in one L2.  With fewer, ranks are
 // dealt to the XCDs that share a head 8 neighbours at a time, because neighbours read the same keys (windowed prompts of one
-// kv head 121 -> 101 us; 4 to 32 neighbours measure the same).
+// kv head 121 -> 103 us; 4 to 32 neighbours measure the same).
 __device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
     constexpr int NEIGHBOURS = 8;
     const int share = kv_heads % 8 == 0 ? 1 : kv_heads % 4 == 0 ? 2 : kv_heads % 2 == 0 ? 4 : 8, block = share * NEIGHBOURS;
@@ -203,7 +208,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     }
     // page of the 16 keys from `key0`, or -1
     const auto page_at = [&](int key0) { return key0 <= last ? page_of(a.c, b, key0 >> a.c.page_shift) : -1; };
-    int pages[Load::PIECES] = {}, my_page = -1;                         // of the tile after the next
+    int pages[Load::PIECES] = {}, my_page = -1;                      // of the tile after the next
     const auto look_up = [&](int u) {
         if constexpr (PAGED) {
             if (u >= u1) return;
@@ -216,9 +221,10 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             my_page = page_at(key + 16 * (tid % (2 * GROUPS) >> 1));
         }
     };
-    // FP16: element offsets of the lane's pieces in a tile (strides are below 2^24)
+    // FP16: byte offsets of the lane's pieces in a tile (strides are below 2^24)
     const uint32_t k_next = 512 / (D / 8) * a.k_stride, v_next = 512 / (D / 8) * a.v_stride;
-    const uint32_t k_lane = 2 * (tid / (D / 8) * (uint32_t)a.k_stride + tid % (D / 8) * 8), v_lane = 2 * (tid / (D / 8) * (uint32_t)a.v_stride + tid % (D / 8) * 8);
+    const uint32_t k_lane = 2 * (tid / (D / 8) * (uint32_t)a.k_stride + tid % (D / 8) * 8);
+    const uint32_t v_lane = 2 * (tid / (D / 8) * (uint32_t)a.v_stride + tid % (D / 8) * 8);
     const auto fetch = [&](Load& t, int u) {
         const int key = key_of(u);
         if constexpr (PAGED) {
@@ -235,8 +241,11 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         } else {
             // a tile's base is the same for all lanes; rows past the last key read as zero
             const int most = u < u1 ? min(last - key, BK - 1) : -1;
-            const auto kb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.k) + (size_t)(rows.first + key) * a.k_stride + (size_t)head * D, 0, most < 0 ? 0 : 2 * (most * (int)a.k_stride + D), 0x00027000);
-            const auto vb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.v) + (size_t)(rows.first + key) * a.v_stride + (size_t)head * D, 0, most < 0 ? 0 : 2 * (most * (int)a.v_stride + D), 0x00027000);
+            const auto rows_from = [&](const uint16_t* x, size_t stride) {
+                return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(x) + (size_t)(rows.first + key) * stride + (size_t)head * D, 0,
+                                                         most < 0 ? 0 : 2 * (most * (int)stride + D), 0x00027000);
+            };
+            const auto kb = rows_from(a.k, a.k_stride), vb = rows_from(a.v, a.v_stride);
 #pragma unroll
             for (int i = 0; i < Load::PIECES; i++)
                 t.k[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, k_lane + i * k_next, 0, 0));
@@ -412,6 +421,9 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
                 for (int r = 0; r < AR; r++) o[i][r] *= f;
         }
+        // The wave that feeds the matrix cores goes before the one that is elsewhere in its tile: 2% at D = 128, nothing at 256; at
+        // 64, where the products are short against the rest, it costs 4%.
+        if constexpr (D > 64) __builtin_amdgcn_s_setprio(1);
         v8h p[FRAGS];
 #pragma unroll
         for (int f = 0; f < FRAGS; f++) {
@@ -434,16 +446,17 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             for (int i = 0; i < NDT; i++) o[i] = Product<RW>::mul(value_frag(buf, i, f), p[f], o[i]);
         }
         // The first values are read while the first weights are computed; then every product is followed by the reads of one
-        // VALUES_AHEAD further on and a share of the next fragment's exponentials, which run beside the matrix cores.
+        // READ_AHEAD further on and a share of the next fragment's exponentials, which run beside the matrix cores.
         constexpr int PER_FRAG = 28, SHARE = (PER_FRAG + NDT - 1) / NDT, PRODUCTS = FRAGS * NDT;
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * VALUES_AHEAD, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * READ_AHEAD, 1);
         __builtin_amdgcn_sched_group_barrier(0x402, PER_FRAG, 1);
 #pragma unroll
         for (int i = 0; i < PRODUCTS; i++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-            if (i < PRODUCTS - VALUES_AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            if (i < PRODUCTS - READ_AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
             if (i < PRODUCTS - NDT) __builtin_amdgcn_sched_group_barrier(0x402, SHARE, 1);
         }
+        if constexpr (D > 64) __builtin_amdgcn_s_setprio(0);
         if constexpr (!PAGED) {
             if (s_odd[buf] == u + 1) {
                 // The values that are not finite are zero in LDS (stash).  Every row that puts weight on such a key is marked:
