@@ -114,7 +114,7 @@ void attention_step_kernel(const PagedAttnArgs a, const int splits, const int ro
     const int R = min(rows.count * group - tile * STEP_ROWS, STEP_ROWS);       // rows of this tile
     // a ragged batch: sequences with more rows are the chunk kernel's
     if (R <= 0 || (a.cu && rows.count * group > STEP_ROWS)) return;
-    const int context = min(a.contexts[b], a.c.table_width << a.c.page_shift);
+    const int context = context_of(a, b);
     const int row = tile * STEP_ROWS + min(n, R - 1);                          // lanes past the last row repeat it
     const int token = rows.first + row / group, qh = head * group + row % group;
     const int pos = context - rows.count + row / group;

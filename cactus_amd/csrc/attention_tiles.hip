@@ -161,7 +161,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     const int R = tile < 0 ? 0 : min(rows.count * group - tile * TILE_ROWS, TILE_ROWS);
     if (R <= 0 || (PAGED && rows.count * group <= a.min_rows)) return;
     int context = rows.count;
-    if (PAGED) context = min(a.contexts[b], a.c.table_width << a.c.page_shift);
+    if (PAGED) context = context_of(a, b);
     const int pos0 = context - rows.count;                    // position of the sequence's first row
     const auto pos_of = [&](int r) { return pos0 + (tile * TILE_ROWS + r) / group; };
     const int row = min(wave * RW + n, R - 1);                       // lanes past the last row repeat it

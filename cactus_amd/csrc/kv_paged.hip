@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) void read_paged_kernel(const PagedReadArgs a) 
     const int row = (int)(at / chunks), piece = (int)(at % chunks), h = piece / (D / 16), d = piece % (D / 16) * 16;
     while (b < a.batch && row >= a.cu[b + 1]) b++;
     if (b >= a.batch || row < a.cu[b]) return;
-    const long long token = (long long)a.starts[b] + (row - a.cu[b]);
+    const long long token = (long long)a.starts[b] + row - a.cu[b];
     const int page = token < 0 || (token >> a.c.page_shift) >= a.c.table_width ? -1 : page_of(a.c, b, (int)(token >> a.c.page_shift));
     const size_t ph = (size_t)max(page, 0) * a.c.kv_heads + h;
     const size_t src = ((ph << a.c.page_shift) + (size_t)(token & ((1 << a.c.page_shift) - 1))) * D + d;

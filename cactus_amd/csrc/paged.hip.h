@@ -50,6 +50,12 @@ __device__ __forceinline__ int page_of(const PagedCache& c, int b, int i) {
     return p >= 0 && p < c.num_pages ? p : -1;
 }
 
+// Tokens of sequence b that its table can hold.  The lengths are device data that nobody checked: between 0 and 2^30, positions
+// and their differences stay in an int.
+__device__ __forceinline__ int context_of(const PagedAttnArgs& a, int b) {
+    return min(max(a.contexts[b], 0), a.c.table_width << a.c.page_shift);
+}
+
 // The key tiles that rows at positions first .. last see: `sinks` tiles from key 0, then tile `first` and on.
 struct TilePlan {
     int sinks, first, tiles;

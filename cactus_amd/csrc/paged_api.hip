@@ -65,6 +65,10 @@ const char* bad_batch(const int32_t* cu, size_t batch, size_t tokens) {
     return nullptr;
 }
 
+// workgroups of a launch: a grid holds less than 2^32 threads, 512 to a workgroup at most
+constexpr size_t MAX_ITEMS = size_t(1) << 23;
+const char* too_many = "too many rows for one launch";
+
 const char* bad_groups(size_t q_heads, size_t kv_heads) {
     if (q_heads == 0 || kv_heads == 0 || q_heads % kv_heads != 0 || q_heads > MAX_HEADS)
         return "num_q_heads must be a multiple of the kv heads, at most 4096";
@@ -200,6 +204,7 @@ int cactus_hip_kv_read_paged_f16_dev(const cactus_hip_paged_kv* cache, const int
     REFUSE_IF(bad_batch(cu_seqlens, batch, rows));
     if (!k_output || !v_output || !aligned16(k_output) || !aligned16(v_output))
         return refuse(who, "outputs must be 16-byte aligned");
+    if (rows * cache->kv_heads * (cache->head_dim / 16) >= size_t(1) << 32) return refuse(who, too_many);
     PagedReadArgs a{view(*cache, block_tables, table_width), starts, cu_seqlens, (int)batch, (int)rows, k_output, v_output};
     return launched(who, launch_kv_read_paged((int)cache->head_dim, a, (hipStream_t)stream));
 }
@@ -223,6 +228,7 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
     REFUSE_IF(bad_batch(cu_seqlens, batch, tokens));
     REFUSE_IF(bad_groups(num_q_heads, cache->kv_heads));
     REFUSE_IF(bad_window(window, sink));
+    if (tokens * (num_q_heads / cache->kv_heads) > MAX_ROWS * 8) return refuse(who, too_many);
     if (!context_lens) return refuse(who, "null context_lens");
     REFUSE_IF(bad_rows(q, q_stride, num_q_heads, cache->head_dim));
     REFUSE_IF(bad_rows(output, num_q_heads * cache->head_dim, num_q_heads, cache->head_dim));
@@ -244,7 +250,7 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
     const PagedPlan p = paged_plan(*cache, batch, tokens, max_context, num_q_heads, window, sink, cu_seqlens == nullptr);
     if (p.bytes() > 0 && (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace)))
         return refuse(who, "workspace missing, too small or not 16-byte aligned");
-    if (p.items() > 0x7fffffff) return refuse(who, "too many rows for one launch");
+    if (p.items() >= MAX_ITEMS) return refuse(who, too_many);
     a.work = static_cast<float*>(workspace);
     if (p.by_step) {
         a.work_rows = p.step.rows;
@@ -269,6 +275,7 @@ int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride,
     REFUSE_IF(bad_batch(cu_seqlens, batch, tokens));
     REFUSE_IF(bad_groups(num_q_heads, num_kv_heads));
     REFUSE_IF(bad_window(window, sink));
+    if (tokens * (num_q_heads / num_kv_heads) > MAX_ROWS * 8) return refuse(who, too_many);
     REFUSE_IF(bad_rows(q, q_stride, num_q_heads, head_dim));
     REFUSE_IF(bad_rows(k, k_stride, num_kv_heads, head_dim));
     REFUSE_IF(bad_rows(v, v_stride, num_kv_heads, head_dim));
@@ -291,7 +298,7 @@ int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride,
     a.window = reach(window);
     a.sink = reach(sink);
     const TileShape s = tile_shape(head_dim, batch, tokens, 0, num_q_heads, num_kv_heads, window, sink);      // 0: never split
-    if ((size_t)s.slots * num_kv_heads > 0x7fffffff) return refuse(who, "too many rows for one launch");
+    if ((size_t)s.slots * num_kv_heads >= MAX_ITEMS) return refuse(who, too_many);
     return launched(who, launch_attention_tiles((int)head_dim, false, a, s, (hipStream_t)stream));
 }
 

@@ -691,3 +691,143 @@ def test_python_refuses(P):
         P.attention(torch.zeros((1, 3, 64), dtype=torch.float16, device="cuda"), kv, t, one)
     with pytest.raises(Exception, match="one row per sequence"):
         P.attention(torch.zeros((2, 2, 64), dtype=torch.float16, device="cuda"), kv, t, one)
+
+
+# ------------------------------------------------------------------------------------------- what a caller may hand over
+
+@pytest.mark.parametrize("news", [[1, 1, 1, 1], [40, 1, 70, 3]])
+def test_lengths_that_are_not_lengths(P, news):
+    """Context lengths are device data: below zero they are zero, above the table they end with it."""
+    gen = torch.Generator().manual_seed(9)
+    D, Hq, Hkv, page = 64, 4, 2, 16
+    kv = [x.cuda() for x in random_cache(gen, 40, Hkv, page, D)]
+    t = torch.randperm(40, generator=gen).int().reshape(4, 10).cuda()
+    q = torch.randn((sum(news), Hq, D), generator=gen).half().cuda()
+    cu = R.offsets(news).cuda() if news != [1, 1, 1, 1] else None
+    for window, sink in ((0, 0), (30, 4), ((1 << 31) - 1, (1 << 31) - 1)):
+        a = P.attention(q, kv, t, i32([-(1 << 31), -7, (1 << 31) - 1, 90]).cuda(), cu_seqlens=cu, window=window, sink=sink)
+        b = P.attention(q, kv, t, i32([0, 0, 160, 90]).cuda(), cu_seqlens=cu, window=window, sink=sink)
+        assert torch.equal(a, b)
+        assert not a[:news[0] + news[1]].any()
+        if window > 30:
+            assert torch.equal(a, P.attention(q, kv, t, i32([0, 0, 160, 90]).cuda(), cu_seqlens=cu))
+
+
+def test_sequence_offsets_that_are_not_offsets(P):
+    """cu_seqlens is device data: whatever it holds, reads and writes stay inside the rows, and the calls end."""
+    gen = torch.Generator().manual_seed(10)
+    D, Hq, Hkv, page, T = 64, 4, 2, 16, 200
+    kv = [x.cuda() for x in random_cache(gen, 60, Hkv, page, D)]
+    t = torch.randperm(60, generator=gen).int().reshape(4, 15).cuda()
+    rows = lambda h: torch.randn((T, h, D), generator=gen).half().cuda()  # noqa: E731
+    q, k, v = rows(Hq), rows(Hkv), rows(Hkv)
+    guard = torch.full((T + 400, Hq, D), 3.0, dtype=torch.float16, device="cuda")
+    out = guard[200:200 + T]
+    for bad in ([0, 90, 40, 150, 60], [50, 1 << 30, -5, (1 << 31) - 1, -(1 << 31)], [200, 150, 100, 50, 0], [-9, -8, -7, -6, -5]):
+        cu = i32(bad).cuda()
+        P.attention_ragged(q, k, v, cu, out=out)
+        P.attention(q, kv, t, i32([100, 240, 3, 77]).cuda(), cu_seqlens=cu, out=out)
+        P.kv_append(k, v, kv, t, i32([0, 20, 5, 1000]).cuda(), 1e4, cu_seqlens=cu, q=q, out_q=out)
+        k2, v2 = guard[:0].new_full((T + 2, Hkv, D), 3.0), guard[:0].new_full((T + 2, Hkv, D), 3.0)
+        P.kv_read(kv, t, i32([0, 20, -5, 1000]).cuda(), cu, T, out_k=k2[1:-1], out_v=v2[1:-1])
+        torch.cuda.synchronize()
+        assert bool((guard[:200] == 3.0).all()) and bool((guard[200 + T:] == 3.0).all())
+        assert all(bool((x[0] == 3.0).all()) and bool((x[-1] == 3.0).all()) for x in (k2, v2))
+
+
+@pytest.mark.parametrize("D,news,contexts", [(64, [1, 1], [300, 47]), (128, [1, 1], [300, 47]), (256, [1, 1], [300, 47]),
+                                             (64, [70, 40], [300, 120]), (128, [70, 40], [300, 120]), (256, [30, 40], [200, 120])])
+def test_page_scales_far_apart(P, D, news, contexts):
+    """Scales from zero over the smallest that append makes to large ones, side by side.  A weight is rounded to binary16 together
+    with its page's value scale, beside the largest such product: where it is subnormal it is off by 2^-25 of that, times a
+    code of at most 127, for each key."""
+    gen = torch.Generator().manual_seed(11)
+    Hq, Hkv, page = 4, 2, 16
+    used = [(c + page - 1) // page for c in contexts]
+    total = sum(used)
+    kv = list(random_cache(gen, total, Hkv, page, D))
+    pick = lambda xs: torch.tensor(xs)[torch.randint(0, len(xs), (total, Hkv), generator=gen)]  # noqa: E731
+    kv[2], kv[3] = pick([0.0, 1e-10, 1e-3, 0.02, 0.05]), pick([0.0, 1e-10, 1e-4, 0.02, 2.0])
+    t = R.make_tables(gen, used, max(used), total)
+    q = torch.randn((sum(news), Hq, D), generator=gen).half()
+    cu = R.offsets(news)
+    out = P.attention(q.cuda(), [x.cuda() for x in kv], t.cuda(), i32(contexts).cuda(), cu_seqlens=cu.cuda()).cpu().double()
+    for b, (n, c) in enumerate(zip(news, contexts)):
+        k, ok = R.gather(kv[0], kv[2], t[b], page, 0, c)
+        v, _ = R.gather(kv[1], kv[3], t[b], page, 0, c)
+        r = slice(int(cu[b]), int(cu[b]) + n)
+        want, tol = R.attend(q[r], k, v, torch.arange(c - n, c), 0, 0, 0.0, ok)
+        tol = tol + 2.0 ** -25 * 2.0 * 127 * c
+        assert bool(((out[r] - want).abs() <= tol).all()), (b, float(((out[r] - want).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,n", [(64, 8, 2, 1100), (128, 8, 4, 1100), (256, 4, 1, 1100), (64, 12, 3, 2100)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (200, 4)])
+def test_ragged_many_tiles(P, D, Hq, Hkv, n, window, sink):
+    """More row tiles than the order of the workgroups deals out at a time, whatever the number of kv heads; some rows of each
+    sequence are checked."""
+    gen = torch.Generator().manual_seed(n + D)
+    lengths = [3, n, 0, n // 3]
+    T = sum(lengths)
+    q, k, v = (torch.randn((T, h, D), generator=gen).half() for h in (Hq, Hkv, Hkv))
+    cu = R.offsets(lengths)
+    out = P.attention_ragged(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), window=window, sink=sink).cpu().double()
+    assert bool(torch.isfinite(out).all())
+    for b, m in enumerate(lengths):
+        rows = torch.arange(m) if m < 8 else torch.cat([torch.arange(0, m, 61), torch.tensor([m - 1])])
+        base = int(cu[b])
+        want, tol = R.attend(q[base + rows], k[base:base + m], v[base:base + m], rows, window, sink)
+        assert bool(((out[base + rows] - want).abs() <= tol).all()), b
+
+
+@pytest.mark.parametrize("D,page,Hq,Hkv", [(64, 16, 4, 2), (128, 64, 4, 2), (256, 128, 2, 1)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (1500, 4), (2000, 100)])
+def test_chunk_over_a_long_context(P, D, page, Hq, Hkv, window, sink):
+    check_attention(P, D, D, page, Hq, Hkv, [50, 33], [3100, 1700], window, sink)
+
+
+def test_row_strides_of_a_wide_matrix(P):
+    """Rows that are columns of a matrix as wide as a stride may be: offsets inside a tile pass 2^30 bytes."""
+    gen = torch.Generator().manual_seed(12)
+    D, n, stride = 64, 130, (1 << 24) - 8
+    pool = torch.zeros(n * stride // 2, dtype=torch.float32, device="cuda").view(torch.float16)
+    at = [pool.as_strided((n, h, D), (stride, D, 1), o) for h, o in ((2, 0), (1, 1024), (1, 4096))]
+    x = [torch.randn((n, h, D), generator=gen).half().cuda() for h in (2, 1, 1)]
+    for a, b in zip(at, x):
+        a.copy_(b)
+    cu = i32([0, n]).cuda()
+    assert torch.equal(P.attention_ragged(*at, cu), P.attention_ragged(*x, cu))
+
+
+def test_two_graphs_replayed_side_by_side(P):
+    """Two captured calls with scratch of their own, replayed on two streams at once and in turn."""
+    gen = torch.Generator().manual_seed(13)
+    D, Hq, Hkv, page, width = 128, 4, 2, 16, 250
+    kv = [x.cuda() for x in random_cache(gen, 2 * width, Hkv, page, D)]
+    t = torch.randperm(2 * width, generator=gen).int().reshape(2, 1, width).cuda()
+    q = [torch.randn((1, Hq, D), generator=gen).half().cuda() for _ in range(2)]
+    ctx = [i32([3900]).cuda(), i32([2500]).cuda()]
+    graphs, outs = [], []
+    for i in range(2):
+        P.attention(q[i], kv, t[i], ctx[i])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(P.attention(q[i], kv, t[i], ctx[i]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(5):
+        for x in q:
+            x.copy_(torch.randn(x.shape, generator=gen).half())
+        torch.cuda.synchronize()
+        if turn < 3:
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        else:
+            for g in graphs[::-1]:
+                g.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        want = [P.attention(q[i], kv, t[i], ctx[i]) for i in range(2)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn

@@ -124,6 +124,15 @@ def test_empty_calls_do_nothing():
     assert ragged(tokens=0) == 0
 
 
+def test_refuses_more_rows_than_a_launch_holds():
+    many = 1 << 26
+    assert refused(attend(cache(kv_heads=2), cu=A, tokens=many, heads=4096, qs=4096 * 64), "too many rows")
+    assert refused(attend(cache(kv_heads=4096, head_dim=64), batch=1 << 20, tokens=1 << 20, heads=4096, qs=4096 * 64), "too many rows")
+    assert refused(ragged(tokens=many, heads=4096, qs=4096 * 64), "too many rows")
+    assert refused(ragged(tokens=many, heads=64, qs=4096, kv_heads=64, ks=4096, vs=4096), "too many rows")
+    assert refused(read(cache(kv_heads=64), rows=many), "too many rows")
+
+
 def test_python_names_what_is_wrong():
     torch = pytest.importorskip("torch")
     kv = P.empty_pages(4, 2, 64, 16, device="cpu")
