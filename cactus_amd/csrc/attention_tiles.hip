@@ -21,7 +21,7 @@
 //
 // Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 819 TFLOP/s (a large FP16 matrix product reaches
 // 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 91 us, 466.  24 prompts of 17 to 300 tokens,
-// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 53.5 us, 10 of them the join's.
+// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 50.7 us, 10 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
@@ -142,7 +142,9 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     constexpr int BK = Load::BK, KT = BK / RW, GROUPS = BK / 16, FK = 8 * LG, FRAGS = BK / FK, NST = D / (8 * LG), NDT = D / RW, ROW = D * 2;
     typedef typename Product<RW>::Acc Acc;
     __shared__ __attribute__((aligned(1024))) unsigned char s_kv[NG][4][BK * ROW];      // of a group: K, K, V, V
-    __shared__ float s_scales[NG][2][GROUPS][2];
+    // INT8, per 16-key group: factor of the score, (unused), log2 of the value scale, its reciprocal.  A group without a page has
+    // factor 0 and logarithm -inf, which is all the masking it needs.
+    __shared__ __attribute__((aligned(16))) float s_scales[NG][2][GROUPS][4];
     // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
     // tile, not seen whole by every row, that holds such values; s_marks: +inf, -inf, NaN bits of every row's dims
     __shared__ int s_odds[NG][2], s_marked;
@@ -151,7 +153,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // in the group
     const int grp = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int n = lane % RW, h = lane / RW;
-    float(*const s_scale)[GROUPS][2] = s_scales[grp];
+    float(*const s_scale)[GROUPS][4] = s_scales[grp];
     int* const s_odd = s_odds[grp];
     const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
     const int group = a.q_heads / a.kv_heads;
@@ -188,7 +190,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 #pragma unroll
                 for (int e = 0; e < 8; e++) bias += (float)q[s][e];
         }
-        if (PAGED) bias = row_sum<RW>(bias) * -128.0f;
+        if (PAGED) bias = row_sum<RW>(bias) * (-128.0f / 16777216.0f);
     }
     const float c0 = fabsf(a.scale) * LOG2E;
 
@@ -309,7 +311,12 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 *reinterpret_cast<v4i*>(&s_kv[0][2 + buf][i * STEP_BYTES] + v_to) = t.v[i];
             }
         }
-        if (PAGED && tid < 2 * GROUPS) s_scale[buf][tid >> 1][tid & 1] = t.page < 0 ? -1.0f : fmaxf(t.scale, 0.0f);
+        if (PAGED && tid < 2 * GROUPS) {         // worked out once here, not by every wave
+            const float x = t.page < 0 ? 0.0f : fmaxf(t.scale, 0.0f), v = fmaxf(x, 1e-20f);
+            const v2f two = tid & 1 ? v2f{t.page < 0 ? -INFINITY : __log2f(v), t.page < 0 ? 0.0f : __builtin_amdgcn_rcpf(v)}
+                                    : v2f{x * c0 * 16777216.0f, 0.0f};
+            *reinterpret_cast<v2f*>(&s_scale[buf][tid >> 1][2 * (tid & 1)]) = two;
+        }
     };
 
     float m = -1e30f, l = 0.0f;
@@ -361,17 +368,14 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         __builtin_amdgcn_sched_group_barrier(0x008, READ_AHEAD, 0);
         const auto group_of = [](int t, int r) { return (RW * t + QUAD * (r >> 2)) / 16; };      // 16-key group of a score
         float inv_vs[GROUPS];
-        bool live[GROUPS];
         if constexpr (PAGED) {
             float up[GROUPS], add[GROUPS];
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
-                const float ks = s_scale[buf][g][0], v0 = s_scale[buf][g][1], vs = fmaxf(v0, 1e-20f);
-                live[g] = v0 >= 0.0f;
-                const float c = c0 * ks;
-                up[g] = c * 16777216.0f;
-                add[g] = fmaf(c, bias, __log2f(vs));
-                inv_vs[g] = 1.0f / vs;
+                const v4f x = *reinterpret_cast<const v4f*>(s_scale[buf][g]);
+                up[g] = x[0];
+                add[g] = fmaf(x[0], bias, x[2]);
+                inv_vs[g] = x[3];
             }
 #pragma unroll
             for (int t = 0; t < KT; t++)
@@ -396,13 +400,6 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                         const int j = RW * t + QUAD * (r >> 2) + (r & 3);
                         s[t][r] = j >= from || j < sinks ? s[t][r] : -INFINITY;
                     }
-            }
-            if constexpr (PAGED) {
-#pragma unroll
-                for (int t = 0; t < KT; t++)
-#pragma unroll
-                    for (int r = 0; r < AR; r++)
-                        if (!live[group_of(t, r)]) s[t][r] = -INFINITY;
             }
         }
         float top = -INFINITY;
@@ -511,13 +508,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             const bool seen = u < seen_hi && (u >= seen_lo || u < plan.sinks) && (NG == 1 || u < u1);
             if (!seen && u + NG < u1) fetch(t, u + NG);
             if (seen) {
-                bool whole = (u >= whole_lo && u < whole_hi) || u < whole_sinks;
-                if constexpr (PAGED) {
-#pragma unroll
-                    for (int g = 0; g < GROUPS; g++) whole = whole && s_scale[buf][g][1] >= 0.0f;
-                    whole = __builtin_amdgcn_readfirstlane(whole);
-                }
-                compute(buf, t, u, whole);
+                compute(buf, t, u, (u >= whole_lo && u < whole_hi) || u < whole_sinks);
             }
             look_up(u + 2 * NG);
             if (u + NG < u1) stash(other, t, u + NG);
