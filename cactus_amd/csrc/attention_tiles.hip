@@ -21,7 +21,7 @@
 //
 // Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 819 TFLOP/s (a large FP16 matrix product reaches
 // 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 91 us, 466.  24 prompts of 17 to 300 tokens,
-// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 50.7 us, 10 of them the join's.
+// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 48.5 us, 10 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
@@ -142,8 +142,8 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     constexpr int BK = Load::BK, KT = BK / RW, GROUPS = BK / 16, FK = 8 * LG, FRAGS = BK / FK, NST = D / (8 * LG), NDT = D / RW, ROW = D * 2;
     typedef typename Product<RW>::Acc Acc;
     __shared__ __attribute__((aligned(1024))) unsigned char s_kv[NG][4][BK * ROW];      // of a group: K, K, V, V
-    // INT8, per 16-key group: factor of the score, (unused), log2 of the value scale, its reciprocal.  A group without a page has
-    // factor 0 and logarithm -inf, which is all the masking it needs.
+    // INT8, per 16-key group: factor of the score, (unused), log2 of the value scale, its reciprocal.  A group without a page has the
+    // logarithm -inf, which is all the masking it needs.  The factor is above zero, so that a masked score stays -inf.
     __shared__ __attribute__((aligned(16))) float s_scales[NG][2][GROUPS][4];
     // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
     // tile, not seen whole by every row, that holds such values; s_marks: +inf, -inf, NaN bits of every row's dims
@@ -314,7 +314,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         if (PAGED && tid < 2 * GROUPS) {         // worked out once here, not by every wave
             const float x = t.page < 0 ? 0.0f : fmaxf(t.scale, 0.0f), v = fmaxf(x, 1e-20f);
             const v2f two = tid & 1 ? v2f{t.page < 0 ? -INFINITY : __log2f(v), t.page < 0 ? 0.0f : __builtin_amdgcn_rcpf(v)}
-                                    : v2f{x * c0 * 16777216.0f, 0.0f};
+                                    : v2f{fmaxf(x * c0 * 16777216.0f, 1e-30f), 0.0f};
             *reinterpret_cast<v2f*>(&s_scale[buf][tid >> 1][2 * (tid & 1)]) = two;
         }
     };
@@ -367,9 +367,8 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
         }
         __builtin_amdgcn_sched_group_barrier(0x008, READ_AHEAD, 0);
         const auto group_of = [](int t, int r) { return (RW * t + QUAD * (r >> 2)) / 16; };      // 16-key group of a score
-        float inv_vs[GROUPS];
+        float inv_vs[GROUPS], up[GROUPS], add[GROUPS];       // INT8: a weight's exponent is score * up + add of its group
         if constexpr (PAGED) {
-            float up[GROUPS], add[GROUPS];
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
                 const v4f x = *reinterpret_cast<const v4f*>(s_scale[buf][g]);
@@ -377,10 +376,6 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 add[g] = fmaf(x[0], bias, x[2]);
                 inv_vs[g] = x[3];
             }
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int r = 0; r < AR; r++) s[t][r] = fmaf(s[t][r], up[group_of(t, r)], add[group_of(t, r)]);
         }
         if (!whole) {
             // a score's key against the row's own key, its first window key and the sinks
@@ -403,12 +398,24 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             }
         }
         float top = -INFINITY;
+        if constexpr (PAGED) {
+            float most[GROUPS];
 #pragma unroll
-        for (int t = 0; t < KT; t++)
+            for (int g = 0; g < GROUPS; g++) most[g] = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < AR; r += 2) top = fmaxf(fmaxf(s[t][r], s[t][r + 1]), top);
-        top = row_max<RW>(top);
-        if (!PAGED) top *= c0;
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < AR; r += 2) most[group_of(t, r)] = fmaxf(fmaxf(s[t][r], s[t][r + 1]), most[group_of(t, r)]);
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) top = fmaxf(top, fmaf(most[g], up[g], add[g]));
+            top = row_max<RW>(top);
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int r = 0; r < AR; r += 2) top = fmaxf(fmaxf(s[t][r], s[t][r + 1]), top);
+            top = row_max<RW>(top) * c0;
+        }
         if (__any(top > m + 8.0f)) {
             const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
             m = to;
@@ -417,6 +424,10 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
             for (int i = 0; i < NDT; i++)
 #pragma unroll
                 for (int r = 0; r < AR; r++) o[i][r] *= f;
+        }
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) add[g] -= m;
         }
         // The wave that feeds the matrix cores goes before the one that is elsewhere in its tile: 2% at D = 128, nothing at 256; at
         // 64, where the products are short against the rest, it costs 4%.
@@ -429,7 +440,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
                 const int quad = 2 * f + half, t = quad / (AR / 4), r0 = quad % (AR / 4) * 4;
                 float w[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(PAGED ? s[t][r0 + e] - m : fmaf(s[t][r0 + e], c0, -m));
+                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(PAGED ? fmaf(s[t][r0 + e], up[group_of(t, r0)], add[group_of(t, r0)]) : fmaf(s[t][r0 + e], c0, -m));
                 const float sum = (w[0] + w[1]) + (w[2] + w[3]);
                 l = PAGED ? fmaf(sum, inv_vs[group_of(t, r0)], l) : l + sum;
 #pragma unroll
