@@ -21,7 +21,7 @@
 //
 // Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 819 TFLOP/s (a large FP16 matrix product reaches
 // 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 91 us, 466.  24 prompts of 17 to 300 tokens,
-// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 48.5 us, 10 of them the join's.
+// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 47.4 us, 10 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
@@ -131,10 +131,28 @@ __device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
     return slots - 1 - rank;
 }
 
+// Key splits of this batch, at most `most`.  RESIDENT workgroups (two waves per SIMD) fill the chip, and a few more cost a second
+// round: three chunks with 80 row tiles x heads take 47.4 us in 6 splits (480 workgroups), 50.2 in 5 and 62 in 7.  How many row
+// tiles a batch has depends on lengths that only the device knows: up to 64 sequences a wave counts them (1 us of the 47.4); for
+// more the host goes by the largest number there can be.
+constexpr int RESIDENT = 512, COUNTED = 64;
+__device__ __forceinline__ int splits_of(const PagedAttnArgs& a, int most, int group, int size) {
+    if (most == 1 || a.batch > COUNTED) return most;
+    const int lane = threadIdx.x & 63, n = lane < a.batch ? rows_of(a.cu, lane, a.tokens).count * group : 0;
+    int v = n > a.min_rows ? (n + size - 1) / size : 0;
+    v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);        // quad_perm [1,0,3,2]
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);        // quad_perm [2,3,0,1]
+    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);       // row_half_mirror
+    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);       // row_mirror: a row of 16 has its sum
+    const int tiles = (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
+                      (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+    return min(max(RESIDENT / max(tiles * a.kv_heads, 1), 1), most);
+}
+
 // NG: groups of four waves.  Two groups take every second key tile each and join their (maximum, sum, output) at the end.
 template <int D, bool PAGED, int NG>
 __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2)))
-void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int slots) {
+void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const int slots) {
     using Load = TileLoad<D, PAGED>;
     // RW rows a wave, lane n + RW h.  An accumulator holds AR values of a lane, quads of four neighbouring keys (dims): key (dim)
     // QUAD (r / 4) + 4 h + r % 4 of a tile of RW.  Two quads make the eight contracted keys of a lane: FRAGS fragments of FK keys.
@@ -155,8 +173,10 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
     const int n = lane % RW, h = lane / RW;
     float(*const s_scale)[GROUPS][4] = s_scales[grp];
     int* const s_odd = s_odds[grp];
-    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
-    const int group = a.q_heads / a.kv_heads;
+    const int group = a.q_heads / a.kv_heads, splits = PAGED ? splits_of(a, most_splits, group, TILE_ROWS) : 1;
+    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads;
+    if (id >= slots * a.kv_heads) return;
+    const int slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
     const Rows rows = rows_of(a.cu, b, a.tokens);
@@ -612,10 +632,12 @@ void attention_tile_kernel(const PagedAttnArgs a, const int splits, const int sl
 
 // joins the splits of a tile's rows: a wave per row, lanes = dims
 template <int D>
-__global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int splits, const int slots) {
+__global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int most_splits, const int slots) {
     constexpr int TILE_ROWS = tile_rows(D);
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = blockIdx.x, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads), group = a.q_heads / a.kv_heads;
+    const int splits = splits_of(a, most_splits, group, TILE_ROWS);
+    if (splits == 1) return;                     // the tile kernel wrote the rows itself
     const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
     const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
     const Rows rows = rows_of(a.cu, b, a.tokens);
@@ -658,7 +680,8 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 }  // namespace
 
 // A tile kernel's launch: a slot per tile of a sequence's rows and kv head, and key splits where that leaves most of the chip
-// idle: as many as fill it twice over, each with at least 512 keys.
+// idle, each of at least 512 keys.  For up to 64 sequences `splits` is what their smallest number of row tiles would take; the
+// kernel takes less when there are more (splits_of).
 TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
                      size_t window, size_t sink) {
     TileShape s;
@@ -667,7 +690,7 @@ TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_co
     const size_t items = (size_t)s.slots * kv_heads;
     size_t keys = max_context;
     if (window && window + sink + size < keys) keys = window + sink + size;
-    const size_t most = keys / 512, want = 512 / items;
+    const size_t most = keys / 512, tiles = batch <= (size_t)COUNTED ? (rows + size - 1) / size : s.slots, want = RESIDENT / (tiles * kv_heads);
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
     s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
     return s;
