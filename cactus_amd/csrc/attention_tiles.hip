@@ -21,7 +21,7 @@
 //
 // Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 819 TFLOP/s (a large FP16 matrix product reaches
 // 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 91 us, 466.  24 prompts of 17 to 300 tokens,
-// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 47.4 us, 10 of them the join's.
+// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 44.4 us, 8 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
@@ -645,18 +645,37 @@ __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAtt
     if (tile < 0 || orow >= rows.count * group || rows.count * group <= a.min_rows) return;
     constexpr size_t step = (size_t)TILE_ROWS * (D + 2);
     const float* rec = a.work + (size_t)id * splits * step;
-    float m = -1e30f, l = 0.0f;
-    for (int s = 0; s < splits; s++) m = fmaxf(m, rec[s * step + 2 * row]);
-    constexpr int W = D / 64;
-    float o[W];
+    // Eight records at a time, all requested before the first is used: latency is what there is to hide.  Records that do not exist
+    // are the last one again, with weight 0.
+    constexpr int W = D / 64, AT_ONCE = 8;
+    typedef float Dims __attribute__((ext_vector_type(W)));
+    float m = -1e30f, l = 0.0f, o[W];
 #pragma unroll
     for (int i = 0; i < W; i++) o[i] = 0.0f;
-    for (int s = 0; s < splits; s++) {
-        const float f = __builtin_amdgcn_exp2f(rec[s * step + 2 * row] - m);
-        l = fmaf(rec[s * step + 2 * row + 1], f, l);
-        const float* x = rec + s * step + 2 * TILE_ROWS + (size_t)row * D + lane * W;
+    for (int s0 = 0; s0 < splits; s0 += AT_ONCE) {
+        v2f ml[AT_ONCE];
+        Dims x[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < W; i++) o[i] = fmaf(x[i], f, o[i]);
+        for (int s = 0; s < AT_ONCE; s++) {
+            const float* from = rec + min(s0 + s, splits - 1) * step;
+            ml[s] = *reinterpret_cast<const v2f*>(from + 2 * row);
+            x[s] = *reinterpret_cast<const Dims*>(from + 2 * TILE_ROWS + (size_t)row * D + lane * W);
+        }
+        float to = m;
+#pragma unroll
+        for (int s = 0; s < AT_ONCE; s++) to = fmaxf(to, ml[s][0]);
+        const float back = __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= back;
+#pragma unroll
+        for (int i = 0; i < W; i++) o[i] *= back;
+#pragma unroll
+        for (int s = 0; s < AT_ONCE; s++) {
+            const float f = s0 + s < splits ? __builtin_amdgcn_exp2f(ml[s][0] - m) : 0.0f;
+            l = fmaf(ml[s][1], f, l);
+#pragma unroll
+            for (int i = 0; i < W; i++) o[i] = fmaf(x[s][i], f, o[i]);
+        }
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     uint16_t* out = a.out + ((size_t)(rows.first + orow / group) * a.q_heads + head * group + orow % group) * D + lane * W;
