@@ -4,8 +4,8 @@
 // max(|x|) / 127 of its tokens, q = rne(x / scale).  Bound: HBM for prompts (rows in, INT8 and the q rows out: every byte
 // moves once), launch latency for a decode step.
 //
-// A workgroup takes the part of ONE page that the call writes, either for some kv heads (keys and values: a page's maximum
-// never leaves the workgroup) or for some query heads; the launch cuts the heads finer the fewer pages there are.  D / 16 lanes
+// A workgroup takes the part of ONE page that the call writes, either for some of its items (a kv head's keys or its values: their
+// maximum never leaves the workgroup) or for some query heads; the launch cuts finer the fewer pages there are.  D / 16 lanes
 // hold a row: lane j the 8 elements from 8 j and their rotation partners from D / 2 + 8 j, two 16-byte loads, no exchange for
 // the rotation.  The row slots of a workgroup are (token of the page) x (head): STEP (one row per sequence) gives them all to
 // heads, otherwise tokens come first.  A lane keeps its tokens while it walks the heads, so an angle is computed once per
@@ -135,6 +135,9 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
 
     const int TP = STEP ? 1 : min(P, slots), HP = slots / TP;  // tokens x heads of a pass
     const int ts = slot % TP, hs = slot / TP;
+    // items of a page: its heads' keys, then their values
+    const int item0 = blockIdx.y * a.kv_per_part, items = min(a.kv_per_part, 2 * a.c.kv_heads - item0);
+    const bool turns = a.rotate && ((int)blockIdx.y >= a.kv_parts || item0 < a.c.kv_heads);
     float cs[RPL][8], sn[RPL][8];
     int e[RPL];
     bool live[RPL];
@@ -142,7 +145,7 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
     for (int r = 0; r < RPL; r++) {
         e[r] = STEP ? e_lo : ts + r * TP;
         live[r] = e[r] >= e_lo && e[r] < e_hi;
-        if (a.rotate && live[r]) {
+        if (turns && live[r]) {
             const double pos = (double)(base + e[r]);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -181,14 +184,13 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
 
     const int page = index < a.c.table_width ? page_of(a.c, b, (int)index) : -1;
     if (page < 0) return;
-    const int kv0 = blockIdx.y * a.kv_per_part, kvn = min(a.kv_per_part, a.c.kv_heads - kv0);
     Row16 w{};
     if (a.k_weight) w = load_row<D>(a.k_weight, j);
-    // items: the keys of kvn heads, then their values
-    for (int i0 = 0; i0 < 2 * kvn; i0 += HP) {
-        const int item = i0 + hs;
-        const bool on = item < 2 * kvn, value = item >= kvn;
-        const size_t ph = (size_t)page * a.c.kv_heads + kv0 + (value ? item - kvn : item);
+    for (int i0 = 0; i0 < items; i0 += HP) {
+        const int item = item0 + i0 + hs;
+        const bool on = i0 + hs < items, value = item >= a.c.kv_heads;
+        const int kv_head = value ? item - a.c.kv_heads : item;
+        const size_t ph = (size_t)page * a.c.kv_heads + kv_head;
         float* scale = (value ? a.c.vs : a.c.ks) + ph;
         const float old = on && e_lo > 0 ? *scale : 0.0f;
         if constexpr (!STEP) {
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
 #pragma unroll
         for (int r = 0; r < RPL; r++) {
             if (!on || !live[r]) continue;
-            const size_t row = (size_t)(row0 + e[r]), head = (size_t)(kv0 + (value ? item - kvn : item)) * D;
+            const size_t row = (size_t)(row0 + e[r]), head = (size_t)kv_head * D;
             x[r] = load_row<D>((value ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head, j);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -229,11 +231,12 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
         }
         if (e_lo > 0) {                          // the page held tokens before: bring them to a scale that has grown
             __syncthreads();
-            for (int c = 0; c < min(HP, 2 * kvn - i0); c++) {
+            for (int c = 0; c < min(HP, items - i0); c++) {
                 const float f = s_again[c];
                 if (f < 0.0f) continue;
-                const bool val = i0 + c >= kvn;
-                const size_t first = (((size_t)page * a.c.kv_heads + kv0 + (val ? i0 + c - kvn : i0 + c)) << a.c.page_shift) * D;
+                const int it = item0 + i0 + c;
+                const bool val = it >= a.c.kv_heads;
+                const size_t first = (((size_t)page * a.c.kv_heads + (val ? it - a.c.kv_heads : it)) << a.c.page_shift) * D;
                 int8_t* codes = (val ? a.c.v : a.c.k) + first;
                 for (int i = tid * 16; i < e_lo * D; i += blockDim.x * 16) {
                     v4i q = *reinterpret_cast<const v4i*>(codes + i);
@@ -304,8 +307,8 @@ hipError_t append_paged(const PagedAppendArgs& args, hipStream_t st) {
         const int most = (heads + least - 1) / least, parts = want < (size_t)most ? (int)want : most;
         return (heads + parts - 1) / parts;
     };
-    a.kv_per_part = cut(a.c.kv_heads, at_once / 2 > 1 ? at_once / 2 : 1);
-    a.kv_parts = (a.c.kv_heads + a.kv_per_part - 1) / a.kv_per_part;
+    a.kv_per_part = cut(2 * a.c.kv_heads, at_once);
+    a.kv_parts = (2 * a.c.kv_heads + a.kv_per_part - 1) / a.kv_per_part;
     int q_parts = 0;
     if (a.q) {
         a.q_per_part = cut(a.q_heads, at_once);

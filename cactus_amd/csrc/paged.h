@@ -33,7 +33,7 @@ struct PagedAppendArgs {
     const uint16_t *q_weight, *k_weight;
     float eps;
     int rotate;
-    int kv_per_part, kv_parts, q_per_part;      // heads of a workgroup, workgroups of a page's kv heads (the launcher's)
+    int kv_per_part, kv_parts, q_per_part;      // items of a workgroup, workgroups of a page's items, query heads of one (the launcher's)
     RopeTurns rope;
 };
 hipError_t launch_kv_append_paged(int head_dim, const PagedAppendArgs& a, hipStream_t st);
