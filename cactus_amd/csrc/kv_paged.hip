@@ -11,6 +11,9 @@
 // heads, otherwise tokens come first.  A lane keeps its tokens while it walks the heads, so an angle is computed once per
 // workgroup: in fp64 as turns (pos * theta^(-2i/D) / 2 pi, only the fraction kept), because an fp32 product at position 30000
 // is off by 1e-3; v_sin_f32 / v_cos_f32 take turns and are off by 2^-23 at most (measured).
+// Measured: 7 prompts of 500 to 1900 tokens, 32 + 2 x 8 heads of 64: 27 us = 4.0 TB/s (a large copy reaches 5.15); a step of one
+// sequence 4.7 us, of 256 6.4 us; 5 chunks of 100 to 256 tokens, 4 + 2 x 1 heads of 256 in pages of 128: 11.4 us, a chain of
+// row, maximum, store and requantization in 96 workgroups.
 #include "paged.hip.h"
 
 #include <math.h>
@@ -258,6 +261,7 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
 
 // Read: a lane turns 16 bytes of a token into 32.  A wave walks the 16-byte pieces of its tokens in memory order; it looks up
 // the sequence of its first token and moves on from there.
+// Bound: HBM; 53 MB in 12.4 us = 4.3 TB/s, a few tokens 2.6 us.
 template <int D>
 __global__ __launch_bounds__(256) void read_paged_kernel(const PagedReadArgs a) {
     const int chunks = a.c.kv_heads * (D / 16);              // 16-byte pieces of a token, keys or values
