@@ -19,9 +19,9 @@
 // with the score's fma), values as b 2^-9.  Page scales enter as in attention_paged.hip.
 // Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count); everything else is fp32.
 //
-// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 819 TFLOP/s (a large FP16 matrix product reaches
-// 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 91 us, 466.  24 prompts of 17 to 300 tokens,
-// D = 64: 19.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 44.3 us, 9 of them the join's.
+// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 83 us, 825 TFLOP/s (a large FP16 matrix product reaches
+// 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 89 us, 475.  24 prompts of 17 to 300 tokens,
+// D = 64: 18.2 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 42.6 us, 9 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
@@ -131,22 +131,50 @@ __device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
     return slots - 1 - rank;
 }
 
-// Key splits of this batch, at most `most`.  RESIDENT workgroups (two waves per SIMD) fill the chip, and a few more cost a second
-// round: three chunks with 80 row tiles x heads take 47.4 us in 6 splits (480 workgroups), 50.2 in 5 and 62 in 7.  How many row
-// tiles a batch has depends on lengths that only the device knows: up to 64 sequences a wave counts them (1 us of the 47.4); for
-// more the host goes by the largest number there can be.
+// Which tile of whose rows a workgroup takes, and how many splits its keys have.
+//
+// How many row tiles a batch has depends on lengths that only the device knows.  For up to COUNTED sequences a wave counts them, a
+// lane per sequence, and numbers them without gaps; RESIDENT workgroups (two waves per SIMD) fill the chip, and a few more cost a
+// second round (three chunks with 80 row tiles x heads take 47.4 us in 6 splits = 480 workgroups, 50.2 in 5 and 62 in 7), so the keys
+// get the largest number of splits that stays within them.  Above, slots lie as slot_begin has them and the host's `most` goes
+// by the largest number of tiles there can be.
 constexpr int RESIDENT = 512, COUNTED = 64;
-__device__ __forceinline__ int splits_of(const PagedAttnArgs& a, int most, int group, int size) {
-    if (most == 1 || a.batch > COUNTED) return most;
+struct Place {
+    int b, tile, split, splits, id;      // id: of the (tile, head) pair; tile < 0: nothing to do
+};
+template <bool JOIN>
+__device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int most, int slots, int group, int size) {
+    Place p;
+    p.tile = -1;
+    if (a.batch > COUNTED) {
+        p.splits = most;
+        p.id = JOIN ? block : block / most;
+        p.split = JOIN ? 0 : block % most;
+        const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, size, 1); };
+        const int slot = slot_of(p.id / a.kv_heads, slots, a.kv_heads);
+        p.b = owner_of(slot, a.batch, begin);
+        if (rows_of(a.cu, p.b, a.tokens).count * group > a.min_rows) p.tile = slot - begin(p.b);
+        return p;
+    }
     const int lane = threadIdx.x & 63, n = lane < a.batch ? rows_of(a.cu, lane, a.tokens).count * group : 0;
-    int v = n > a.min_rows ? (n + size - 1) / size : 0;
-    v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);        // quad_perm [1,0,3,2]
-    v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);        // quad_perm [2,3,0,1]
-    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);       // row_half_mirror
-    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);       // row_mirror: a row of 16 has its sum
-    const int tiles = (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
-                      (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
-    return min(max(RESIDENT / max(tiles * a.kv_heads, 1), 1), most);
+    const int count = n > a.min_rows ? (n + size - 1) / size : 0;
+    int upto = count;                    // tiles of the lane's sequence and those before it
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xF, 0xF, true);       // row_shr:1, 2, 4, 8
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xF, 0xF, true);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, true);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, true);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xA, 0xF, true);       // row_bcast:15 into rows 1 and 3
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xC, 0xF, true);       // row_bcast:31 into rows 2 and 3
+    const int tiles = __builtin_amdgcn_readlane(upto, 63), pairs = min(tiles, RESIDENT) * a.kv_heads;
+    p.splits = min(max(RESIDENT / max(pairs, 1), 1), most);
+    p.id = JOIN ? block : block / p.splits;
+    p.split = JOIN ? 0 : block % p.splits;
+    const int rank = p.id / a.kv_heads;
+    if (rank >= tiles) return p;
+    const int slot = slot_of(rank, tiles, a.kv_heads);
+    p.b = min(__popcll(__ballot(upto <= slot)), a.batch - 1);
+    p.tile = slot - __builtin_amdgcn_readlane(upto - count, p.b);
+    return p;
 }
 
 // NG: groups of four waves.  Two groups take every second key tile each and join their (maximum, sum, output) at the end.
@@ -173,15 +201,13 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
     const int n = lane % RW, h = lane / RW;
     float(*const s_scale)[GROUPS][4] = s_scales[grp];
     int* const s_odd = s_odds[grp];
-    const int group = a.q_heads / a.kv_heads, splits = PAGED ? splits_of(a, most_splits, group, TILE_ROWS) : 1;
-    const int split = blockIdx.x % splits, id = blockIdx.x / splits, head = id % a.kv_heads;
-    if (id >= slots * a.kv_heads) return;
-    const int slot = slot_of(id / a.kv_heads, slots, a.kv_heads);
-    const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
-    const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
+    const int group = a.q_heads / a.kv_heads;
+    const Place at = place_of<false>(a, blockIdx.x, most_splits, slots, group, TILE_ROWS);
+    const int tile = at.tile, b = at.b, splits = PAGED ? at.splits : 1, split = PAGED ? at.split : 0, head = at.id % a.kv_heads;
+    if (tile < 0) return;
     const Rows rows = rows_of(a.cu, b, a.tokens);
-    const int R = tile < 0 ? 0 : min(rows.count * group - tile * TILE_ROWS, TILE_ROWS);
-    if (R <= 0 || (PAGED && rows.count * group <= a.min_rows)) return;
+    const int R = min(rows.count * group - tile * TILE_ROWS, TILE_ROWS);
+    if (R <= 0) return;
     int context = rows.count;
     if (PAGED) context = context_of(a, b);
     const int pos0 = context - rows.count;                    // position of the sequence's first row
@@ -635,16 +661,15 @@ template <int D>
 __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAttnArgs a, const int most_splits, const int slots) {
     constexpr int TILE_ROWS = tile_rows(D);
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = blockIdx.x, head = id % a.kv_heads, slot = slot_of(id / a.kv_heads, slots, a.kv_heads), group = a.q_heads / a.kv_heads;
-    const int splits = splits_of(a, most_splits, group, TILE_ROWS);
-    if (splits == 1) return;                     // the tile kernel wrote the rows itself
-    const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, TILE_ROWS, 1); };
-    const int b = owner_of(slot, a.batch, begin), tile = slot - begin(b);
-    const Rows rows = rows_of(a.cu, b, a.tokens);
+    const int group = a.q_heads / a.kv_heads;
+    const Place at = place_of<true>(a, blockIdx.x, most_splits, slots, group, TILE_ROWS);
+    if (at.tile < 0 || at.splits == 1) return;       // one split: the tile kernel wrote the rows itself
+    const int tile = at.tile, splits = at.splits, head = at.id % a.kv_heads;
+    const Rows rows = rows_of(a.cu, at.b, a.tokens);
     const int orow = tile * TILE_ROWS + row;
-    if (tile < 0 || orow >= rows.count * group || rows.count * group <= a.min_rows) return;
+    if (orow >= rows.count * group) return;
     constexpr size_t step = (size_t)TILE_ROWS * (D + 2);
-    const float* rec = a.work + (size_t)id * splits * step;
+    const float* rec = a.work + (size_t)at.id * splits * step;
     // Eight records at a time, all requested before the first is used: latency is what there is to hide.  Records that do not exist
     // are the last one again, with weight 0.
     constexpr int W = D / 64, AT_ONCE = 8;
@@ -685,33 +710,36 @@ __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAtt
 
 template <int D, bool PAGED>
 hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
-    const size_t items = (size_t)s.slots * a.kv_heads;
     if (D < 256 && s.groups == 2)
-        attention_tile_kernel<D, PAGED, D < 256 ? 2 : 1><<<dim3((unsigned)(items * s.splits)), dim3(512), 0, st>>>(a, s.splits, s.slots);
+        attention_tile_kernel<D, PAGED, D < 256 ? 2 : 1><<<dim3((unsigned)s.blocks), dim3(512), 0, st>>>(a, s.splits, s.slots);
     else
-        attention_tile_kernel<D, PAGED, 1><<<dim3((unsigned)(items * s.splits)), dim3(256), 0, st>>>(a, s.splits, s.slots);
+        attention_tile_kernel<D, PAGED, 1><<<dim3((unsigned)s.blocks), dim3(256), 0, st>>>(a, s.splits, s.slots);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || s.splits == 1) return e;
-    attention_tile_join_kernel<D><<<dim3((unsigned)items, tile_rows(D) / 4), dim3(256), 0, st>>>(a, s.splits, s.slots);
+    attention_tile_join_kernel<D><<<dim3((unsigned)s.joined, tile_rows(D) / 4), dim3(256), 0, st>>>(a, s.splits, s.slots);
     return hipGetLastError();
 }
 
 }  // namespace
 
 // A tile kernel's launch: a slot per tile of a sequence's rows and kv head, and key splits where that leaves most of the chip
-// idle, each of at least 512 keys.  For up to 64 sequences `splits` is what their smallest number of row tiles would take; the
-// kernel takes less when there are more (splits_of).
+// idle, each of at least 512 keys.  Up to COUNTED sequences the kernel chooses the splits (place_of): more than one only while
+// all workgroups are at most RESIDENT, and then at most half as many rows tiles x heads to join.
 TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
                      size_t window, size_t sink) {
     TileShape s;
-    const size_t rows = tokens * (q_heads / kv_heads), size = tile_rows((int)head_dim);
-    s.slots = (int)(batch == 1 ? (rows + size - 1) / size : rows / size + batch);     // slot_begin
+    const size_t rows = tokens * (q_heads / kv_heads), size = tile_rows((int)head_dim), least = (rows + size - 1) / size;
+    s.slots = (int)(batch == 1 ? least : rows / size + batch);                        // slot_begin
     const size_t items = (size_t)s.slots * kv_heads;
     size_t keys = max_context;
     if (window && window + sink + size < keys) keys = window + sink + size;
-    const size_t most = keys / 512, tiles = batch <= (size_t)COUNTED ? (rows + size - 1) / size : s.slots, want = RESIDENT / (tiles * kv_heads);
+    const bool counted = batch <= (size_t)COUNTED;
+    const size_t most = keys / 512, want = RESIDENT / ((counted ? least : s.slots) * kv_heads);
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
     s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
+    s.blocks = counted && s.splits > 1 ? (items > (size_t)RESIDENT ? items : RESIDENT) : items * s.splits;
+    s.records = s.splits == 1 ? 0 : counted ? RESIDENT : s.blocks;
+    s.joined = counted && items > (size_t)RESIDENT / 2 ? RESIDENT / 2 : items;
     return s;
 }
 size_t tile_record_floats(size_t head_dim) { return tile_rows((int)head_dim) * (head_dim + 2); }

@@ -72,11 +72,14 @@ struct StepShape {
 StepShape step_shape(size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
                      bool one_row_each);
 hipError_t launch_attention_step(int head_dim, const PagedAttnArgs& a, const StepShape& s, hipStream_t st);
-// attention_tiles.hip: 128 rows at a time, over the pages or over FP16 rows
+// attention_tiles.hip: 128 rows at a time, over the pages or over FP16 rows.  blocks: workgroups, records: split records, joined:
+// workgroups of the join (times the rows)
 struct TileShape {
     int slots, splits, groups;
+    size_t blocks, records, joined;
 };
-TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink);
+TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
+                     size_t window, size_t sink);
 size_t tile_record_floats(size_t head_dim);
 hipError_t launch_attention_tiles(int head_dim, bool paged, const PagedAttnArgs& a, const TileShape& s, hipStream_t st);
 

@@ -121,8 +121,8 @@ PagedPlan paged_plan(const cactus_hip_paged_kv& c, size_t batch, size_t tokens, 
     }
     if (p.by_tile) {
         p.tile = tile_shape(c.head_dim, batch, tokens, max_context, q_heads, c.kv_heads, window, sink);
-        p.tile_items = (size_t)p.tile.slots * c.kv_heads * p.tile.splits;
-        if (p.tile.splits > 1) p.tile_bytes = p.tile_items * tile_record_floats(c.head_dim) * sizeof(float);
+        p.tile_items = p.tile.blocks;
+        p.tile_bytes = p.tile.records * tile_record_floats(c.head_dim) * sizeof(float);
     }
     return p;
 }
@@ -298,7 +298,7 @@ int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride,
     a.window = reach(window);
     a.sink = reach(sink);
     const TileShape s = tile_shape(head_dim, batch, tokens, 0, num_q_heads, num_kv_heads, window, sink);      // 0: never split
-    if ((size_t)s.slots * num_kv_heads >= MAX_ITEMS) return refuse(who, too_many);
+    if (s.blocks >= MAX_ITEMS) return refuse(who, too_many);
     return launched(who, launch_attention_tiles((int)head_dim, false, a, s, (hipStream_t)stream));
 }
 

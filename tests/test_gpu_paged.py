@@ -831,3 +831,18 @@ def test_two_graphs_replayed_side_by_side(P):
         got = [o.clone() for o in outs]
         want = [P.attention(q[i], kv, t[i], ctx[i]) for i in range(2)]
         assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
+@pytest.mark.parametrize("batch", [2, 17, 63, 64, 65, 130])
+@pytest.mark.parametrize("D,Hq,Hkv,longest", [(64, 4, 2, 150), (128, 2, 1, 200), (256, 8, 1, 20)])
+def test_batches_of_every_size(P, batch, D, Hq, Hkv, longest):
+    """Chunks beside single tokens and sequences that bring nothing; long and short contexts (split keys), prompts too."""
+    gen = torch.Generator().manual_seed(batch + D)
+    news = [int(x) for x in torch.randint(0, 4, (batch,), generator=gen)]
+    for b, n in ((batch // 3, longest), (batch - 1, longest // 2 + 1), (0, 17)):
+        news[b] = n
+    contexts = [n + int(x) for n, x in zip(news, torch.randint(0, 40, (batch,), generator=gen))]
+    contexts[batch // 3] += 1100
+    contexts[batch - 1] += 600
+    check_attention(P, batch, D, 32, Hq, Hkv, news, contexts)
+    check_ragged(P, batch, D, Hq, Hkv, news, 40, 3)
