@@ -134,14 +134,24 @@ __device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
 // Which tile of whose rows a workgroup takes, and how many splits its keys have.
 //
 // How many row tiles a batch has depends on lengths that only the device knows.  For up to COUNTED sequences a wave counts them, a
-// lane per sequence, and numbers them without gaps; RESIDENT workgroups (two waves per SIMD) fill the chip, and a few more cost a
+// lane for every 64th part of the batch, and numbers them without gaps; RESIDENT workgroups (two waves per SIMD) fill the chip, and a few more cost a
 // second round (three chunks with 80 row tiles x heads take 47.4 us in 6 splits = 480 workgroups, 50.2 in 5 and 62 in 7), so the keys
 // get the largest number of splits that stays within them.  Above, slots lie as slot_begin has them and the host's `most` goes
 // by the largest number of tiles there can be.
-constexpr int RESIDENT = 512, COUNTED = 64;
+constexpr int RESIDENT = 512, COUNTED = 1024;
 struct Place {
     int b, tile, split, splits, id;      // id: of the (tile, head) pair; tile < 0: nothing to do
 };
+// sum over lanes 0 .. this one
+__device__ __forceinline__ int sum_upto(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);       // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);       // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);       // row_bcast:31 into rows 2 and 3
+    return v;
+}
 template <bool JOIN>
 __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int most, int slots, int group, int size) {
     Place p;
@@ -156,24 +166,29 @@ __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int
         if (rows_of(a.cu, p.b, a.tokens).count * group > a.min_rows) p.tile = slot - begin(p.b);
         return p;
     }
-    const int lane = threadIdx.x & 63, n = lane < a.batch ? rows_of(a.cu, lane, a.tokens).count * group : 0;
-    const int count = n > a.min_rows ? (n + size - 1) / size : 0;
-    int upto = count;                    // tiles of the lane's sequence and those before it
-    upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xF, 0xF, true);       // row_shr:1, 2, 4, 8
-    upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xF, 0xF, true);
-    upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, true);
-    upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, true);
-    upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xA, 0xF, true);       // row_bcast:15 into rows 1 and 3
-    upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xC, 0xF, true);       // row_bcast:31 into rows 2 and 3
-    const int tiles = __builtin_amdgcn_readlane(upto, 63), pairs = min(tiles, RESIDENT) * a.kv_heads;
+    const int lane = threadIdx.x & 63, per = (a.batch + 63) >> 6;
+    const auto tiles_of = [&](int b) {
+        const int n = b < a.batch ? rows_of(a.cu, b, a.tokens).count * group : 0;
+        return n > a.min_rows ? (n + size - 1) / size : 0;
+    };
+    int count = 0;
+    for (int i = 0; i < per; i++) count += tiles_of(lane * per + i);
+    const int upto = sum_upto(count), tiles = __builtin_amdgcn_readlane(upto, 63), pairs = min(tiles, RESIDENT) * a.kv_heads;
     p.splits = min(max(RESIDENT / max(pairs, 1), 1), most);
     p.id = JOIN ? block : block / p.splits;
     p.split = JOIN ? 0 : block % p.splits;
     const int rank = p.id / a.kv_heads;
     if (rank >= tiles) return p;
     const int slot = slot_of(rank, tiles, a.kv_heads);
-    p.b = min(__popcll(__ballot(upto <= slot)), a.batch - 1);
-    p.tile = slot - __builtin_amdgcn_readlane(upto - count, p.b);
+    const int part = min(__popcll(__ballot(upto <= slot)), 63);
+    p.b = part * per;
+    p.tile = slot - __builtin_amdgcn_readlane(upto - count, part);
+    if (per > 1) {                       // the sequence in the lane's part
+        const int c = lane < per ? tiles_of(p.b + lane) : 0, u = sum_upto(c), i = min(__popcll(__ballot(u <= p.tile)), per - 1);
+        p.tile -= __builtin_amdgcn_readlane(u - c, i);
+        p.b += i;
+    }
+    p.b = min(p.b, a.batch - 1);
     return p;
 }
 
@@ -724,7 +739,7 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 
 // A tile kernel's launch: a slot per tile of a sequence's rows and kv head, and key splits where that leaves most of the chip
 // idle, each of at least 512 keys.  Up to COUNTED sequences the kernel chooses the splits (place_of): more than one only while
-// all workgroups are at most RESIDENT, and then at most half as many rows tiles x heads to join.
+// all workgroups are at most RESIDENT, so that at most half as many row tiles x heads are joined.
 TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
                      size_t window, size_t sink) {
     TileShape s;

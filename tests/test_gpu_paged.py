@@ -846,3 +846,14 @@ def test_batches_of_every_size(P, batch, D, Hq, Hkv, longest):
     contexts[batch - 1] += 600
     check_attention(P, batch, D, 32, Hq, Hkv, news, contexts)
     check_ragged(P, batch, D, Hq, Hkv, news, 40, 3)
+
+
+@pytest.mark.parametrize("batch", [1000, 1024, 1025])
+def test_batches_of_a_thousand(P, batch):
+    gen = torch.Generator().manual_seed(batch)
+    news = [int(x) for x in torch.randint(0, 2, (batch,), generator=gen)]
+    news[0], news[500], news[batch - 1] = 20, 70, 33
+    contexts = [n + int(x) for n, x in zip(news, torch.randint(0, 20, (batch,), generator=gen))]
+    contexts[500] += 1100
+    check_attention(P, batch, 64, 16, 2, 1, news, contexts)
+    check_ragged(P, batch, 64, 2, 1, news)
