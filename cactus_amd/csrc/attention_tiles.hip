@@ -134,11 +134,13 @@ __device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
 // Which tile of whose rows a workgroup takes, and how many splits its keys have.
 //
 // How many row tiles a batch has depends on lengths that only the device knows.  For up to COUNTED sequences a wave counts them, a
-// lane for every 64th part of the batch, and numbers them without gaps; RESIDENT workgroups (two waves per SIMD) fill the chip, and a few more cost a
-// second round (three chunks with 80 row tiles x heads take 47.4 us in 6 splits = 480 workgroups, 50.2 in 5 and 62 in 7), so the keys
-// get the largest number of splits that stays within them.  Above, slots lie as slot_begin has them and the host's `most` goes
-// by the largest number of tiles there can be.
-constexpr int RESIDENT = 512, COUNTED = 1024;
+// lane for every 64th part of the batch, and numbers them without gaps.  As many workgroups as the registers hold (resident) fill the
+// chip, and a few more cost a second round (three chunks with 80 row tiles x heads, D = 128, take 47.4 us in 6 splits = 480
+// workgroups, 50.2 in 5 and 62 in 7; at D = 64 768 take 54 us and 512 60, at 256 103 and 86), so the keys get the largest number of
+// splits that stays within them.  Above, slots lie as slot_begin has them and the host's `most` goes by the largest number of
+// tiles there can be.
+constexpr int resident(int D) { return D == 64 ? 768 : 512; }       // three waves per SIMD, or two
+constexpr int COUNTED = 1024;
 struct Place {
     int b, tile, split, splits, id;      // id: of the (tile, head) pair; tile < 0: nothing to do
 };
@@ -152,8 +154,9 @@ __device__ __forceinline__ int sum_upto(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);       // row_bcast:31 into rows 2 and 3
     return v;
 }
-template <bool JOIN>
-__device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int most, int slots, int group, int size) {
+template <int D, bool JOIN>
+__device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int most, int slots, int group) {
+    constexpr int size = tile_rows(D);
     Place p;
     p.tile = -1;
     if (a.batch > COUNTED) {
@@ -173,8 +176,8 @@ __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int
     };
     int count = 0;
     for (int i = 0; i < per; i++) count += tiles_of(lane * per + i);
-    const int upto = sum_upto(count), tiles = __builtin_amdgcn_readlane(upto, 63), pairs = min(tiles, RESIDENT) * a.kv_heads;
-    p.splits = min(max(RESIDENT / max(pairs, 1), 1), most);
+    const int upto = sum_upto(count), tiles = __builtin_amdgcn_readlane(upto, 63), pairs = min(tiles, resident(D)) * a.kv_heads;
+    p.splits = min(max(resident(D) / max(pairs, 1), 1), most);
     p.id = JOIN ? block : block / p.splits;
     p.split = JOIN ? 0 : block % p.splits;
     const int rank = p.id / a.kv_heads;
@@ -217,7 +220,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
     float(*const s_scale)[GROUPS][4] = s_scales[grp];
     int* const s_odd = s_odds[grp];
     const int group = a.q_heads / a.kv_heads;
-    const Place at = place_of<false>(a, blockIdx.x, most_splits, slots, group, TILE_ROWS);
+    const Place at = place_of<D, false>(a, blockIdx.x, most_splits, slots, group);
     const int tile = at.tile, b = at.b, splits = PAGED ? at.splits : 1, split = PAGED ? at.split : 0, head = at.id % a.kv_heads;
     if (tile < 0) return;
     const Rows rows = rows_of(a.cu, b, a.tokens);
@@ -677,7 +680,7 @@ __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAtt
     constexpr int TILE_ROWS = tile_rows(D);
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = a.q_heads / a.kv_heads;
-    const Place at = place_of<true>(a, blockIdx.x, most_splits, slots, group, TILE_ROWS);
+    const Place at = place_of<D, true>(a, blockIdx.x, most_splits, slots, group);
     if (at.tile < 0 || at.splits == 1) return;       // one split: the tile kernel wrote the rows itself
     const int tile = at.tile, splits = at.splits, head = at.id % a.kv_heads;
     const Rows rows = rows_of(a.cu, at.b, a.tokens);
@@ -739,7 +742,7 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 
 // A tile kernel's launch: a slot per tile of a sequence's rows and kv head, and key splits where that leaves most of the chip
 // idle, each of at least 512 keys.  Up to COUNTED sequences the kernel chooses the splits (place_of): more than one only while
-// all workgroups are at most RESIDENT, so that at most half as many row tiles x heads are joined.
+// they are all resident, so that at most half as many row tiles x heads are joined.
 TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
                      size_t window, size_t sink) {
     TileShape s;
@@ -749,12 +752,12 @@ TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_co
     size_t keys = max_context;
     if (window && window + sink + size < keys) keys = window + sink + size;
     const bool counted = batch <= (size_t)COUNTED;
-    const size_t most = keys / 512, want = RESIDENT / ((counted ? least : s.slots) * kv_heads);
+    const size_t fill = resident((int)head_dim), most = keys / 512, want = fill / ((counted ? least : s.slots) * kv_heads);
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
     s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
-    s.blocks = counted && s.splits > 1 ? (items > (size_t)RESIDENT ? items : RESIDENT) : items * s.splits;
-    s.records = s.splits == 1 ? 0 : counted ? RESIDENT : s.blocks;
-    s.joined = counted && items > (size_t)RESIDENT / 2 ? RESIDENT / 2 : items;
+    s.blocks = counted && s.splits > 1 ? (items > fill ? items : fill) : items * s.splits;
+    s.records = s.splits == 1 ? 0 : counted ? fill : s.blocks;
+    s.joined = counted && items > fill / 2 ? fill / 2 : items;
     return s;
 }
 size_t tile_record_floats(size_t head_dim) { return tile_rows((int)head_dim) * (head_dim + 2); }
