@@ -36,6 +36,7 @@ for _name, (_res, _args) in PAGED_SIGNATURES.items():
 
 # the handle of a device's current stream, without a Stream object around it where torch has the call for that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 _append = H.lib.cactus_hip_kv_append_paged_f16_dev
 _read = H.lib.cactus_hip_kv_read_paged_f16_dev
@@ -80,7 +81,7 @@ def _rows(t, dev, shape, what):
 
 def _output(t, like, dev, shape, what):
     if t is None:
-        return like.new_empty(shape, dtype=torch.float16)
+        return like.new_empty(shape) if like.dtype is torch.float16 else like.new_empty(shape, dtype=torch.float16)
     if t.dtype is not torch.float16 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"paged: {what} must be contiguous float16 {list(shape)} on cuda:{dev}")
     return t
@@ -89,17 +90,18 @@ def _output(t, like, dev, shape, what):
 def _cache(kv, block_tables):
     """(the C description, device number, batch, table width)"""
     k, v, ks, vs = kv
-    shape, dev = k.shape, k.get_device()
+    shape, dev, int8, f32 = k.shape, k.get_device(), torch.int8, torch.float32
     if dev < 0:
         raise ValueError(f"paged: the cache must be on a GPU, not {k.device}")
-    if len(shape) != 4 or k.dtype is not torch.int8 or not k.is_contiguous():
+    if len(shape) != 4 or k.dtype is not int8 or not k.is_contiguous():
         raise ValueError("paged: k pages must be contiguous int8 [pages, kv_heads, page_size, head_dim]")
-    if v.shape != shape or v.dtype is not torch.int8 or v.get_device() != dev or not v.is_contiguous():
+    if v.shape != shape or v.dtype is not int8 or v.get_device() != dev or not v.is_contiguous():
         raise ValueError("paged: v pages must be like the k pages")
     pages, heads, size, dim = shape
-    for s in (ks, vs):
-        if s.dtype is not torch.float32 or s.shape != (pages, heads) or s.get_device() != dev or not s.is_contiguous():
-            raise ValueError("paged: scales must be contiguous float32 [pages, kv_heads] beside the pages")
+    per_head = (pages, heads)
+    if (ks.shape != per_head or vs.shape != per_head or ks.dtype is not f32 or vs.dtype is not f32 or ks.get_device() != dev
+            or vs.get_device() != dev or not ks.is_contiguous() or not vs.is_contiguous()):
+        raise ValueError("paged: scales must be contiguous float32 [pages, kv_heads] beside the pages")
     table = block_tables.shape
     _need(len(table) == 2, "block_tables must be [batch, width]")
     _ints(block_tables, dev, table, "block_tables")
@@ -108,7 +110,7 @@ def _cache(kv, block_tables):
 
 def _call(dev, fn, *args):
     """fn on the device's current stream, with the device current while it runs."""
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
