@@ -11,7 +11,7 @@
 // heads, otherwise tokens come first.  A lane keeps its tokens while it walks the heads, so an angle is computed once per
 // workgroup: in fp64 as turns (pos * theta^(-2i/D) / 2 pi, only the fraction kept), because an fp32 product at position 30000
 // is off by 1e-3; v_sin_f32 / v_cos_f32 take turns and are off by 2^-23 at most (measured).
-// Measured: 7 prompts of 500 to 1900 tokens, 32 + 2 x 8 heads of 64: 27 us = 4.0 TB/s (a large copy reaches 5.15); a step of one
+// Measured: 7 prompts of 500 to 1900 tokens, 32 + 2 x 8 heads of 64: 24 us = 4.5 TB/s (a large copy reaches 5.15); a step of one
 // sequence 4.7 us, of 256 6.4 us; 5 chunks of 100 to 256 tokens, 4 + 2 x 1 heads of 256 in pages of 128: 11.4 us, a chain of
 // row, maximum, store and requantization in 96 workgroups.
 #include "paged.hip.h"
@@ -109,10 +109,10 @@ __device__ __forceinline__ void store_i8(int8_t* __restrict__ row, int j, const 
 
 constexpr int MAX_SLOTS = 256;   // row slots of a workgroup (1024 threads, 4 lanes a row)
 
-template <int D, bool STEP>
+// RPL: tokens a lane holds
+template <int D, bool STEP, int RPL>
 __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArgs a) {
     constexpr int LPR = D / 16;
-    constexpr int RPL = STEP ? 1 : 2;            // tokens a lane holds: the launch picks the workgroup so that 2 are enough
     __shared__ uint32_t s_max[MAX_SLOTS];
     __shared__ float s_again[MAX_SLOTS];         // old / new scale of a head whose earlier tokens are requantized, else -1
 
@@ -301,8 +301,10 @@ hipError_t append_paged(const PagedAppendArgs& args, hipStream_t st) {
     PagedAppendArgs a = args;
     const int P = 1 << a.c.page_shift, LPR = D / 16;
     const bool step = a.cu == nullptr;
-    // as many threads as let two tokens per lane cover a page; a step's row slots are its heads
-    const int threads = step ? 256 : (P * LPR / 2 < 256 ? 256 : P * LPR / 2);
+    // A row slot for every token of the page in 256 threads, else two tokens a lane (a lane's second token costs 35 registers, a
+    // larger workgroup longer waits for each other: prompts of 8000 tokens, 32 heads of 64, pages of 32: 23.4 us with two, 22.2 with
+    // one; 16 heads of 128, pages of 64: 25.2 in 256 threads, 28.1 in 512).  A step's row slots are its heads.
+    const int rpl = P * LPR > 256 ? 2 : 1, threads = step || P * LPR < 256 ? 256 : P * LPR / rpl;
     const size_t pieces = step ? (size_t)a.batch : ((size_t)a.tokens >> a.c.page_shift) + 2 * (size_t)a.batch;
     // heads per workgroup: all of them when there are pages enough to fill the chip (about 1024 workgroups), one pass at least
     const int at_once = step ? 256 / LPR : 1;
@@ -320,9 +322,11 @@ hipError_t append_paged(const PagedAppendArgs& args, hipStream_t st) {
     }
     const dim3 grid((unsigned)pieces, (unsigned)(a.kv_parts + q_parts));
     if (step)
-        append_paged_kernel<D, true><<<grid, dim3(threads), 0, st>>>(a);
+        append_paged_kernel<D, true, 1><<<grid, dim3(threads), 0, st>>>(a);
+    else if (rpl == 1)
+        append_paged_kernel<D, false, 1><<<grid, dim3(threads), 0, st>>>(a);
     else
-        append_paged_kernel<D, false><<<grid, dim3(threads), 0, st>>>(a);
+        append_paged_kernel<D, false, 2><<<grid, dim3(threads), 0, st>>>(a);
     return hipGetLastError();
 }
 
