@@ -21,7 +21,7 @@
 //
 // Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 83 us, 825 TFLOP/s (a large FP16 matrix product reaches
 // 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 89 us, 475.  24 prompts of 17 to 300 tokens,
-// D = 64: 18.2 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 42.6 us, 9 of them the join's.
+// D = 64: 18.2 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 43 us, 8 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
