@@ -857,3 +857,34 @@ def test_batches_of_a_thousand(P, batch):
     contexts[500] += 1100
     check_attention(P, batch, 64, 16, 2, 1, news, contexts)
     check_ragged(P, batch, 64, 2, 1, news)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(16, 1), (40, 2), (64, 1), (130, 1), (14, 7)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_chunks_of_wide_groups(P, D, Hq, Hkv):
+    """More query heads per kv head than a wave or a tile has rows."""
+    check_attention(P, Hq + D, D, 16, Hq, Hkv, [5, 1, 3], [40, 70, 3], 30, 2)
+    check_ragged(P, Hq + D, D, Hq, Hkv, [7, 1, 20], 6, 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sink", [(0, 0), (100, 4)])
+def test_ragged_launches_that_fill_the_chip(P, D, window, sink):
+    """Enough row tiles x kv heads that one group of waves takes all keys of a tile; a value that is not finite spoils the rows that
+    see it, in its dim, and no others."""
+    gen = torch.Generator().manual_seed(D + window)
+    H, lengths = 40, [300, 1400]
+    T = sum(lengths)
+    q, k, v = (torch.randn((T, H, D), generator=gen).half() for _ in range(3))
+    v[300 + 650, :, 5], v[300 + 651, :, 6], k[300 + 1390] = math.nan, math.inf, math.nan
+    cu = R.offsets(lengths)
+    out = P.attention_ragged(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), window=window, sink=sink).cpu().double()
+    for b, m in enumerate(lengths):
+        rows = torch.tensor(sorted({0, 1, m - 1, *range(7, m, 61), *(x for x in (649, 650, 651, 700, 750, 751, 752, 1389) if x < m)}))
+        rows = rows[rows < 1390]
+        base = int(cu[b])
+        want, tol = R.attend(q[base + rows], k[base:base + m], v[base:base + m], rows, window, sink)
+        got, fine = out[base + rows], torch.isfinite(want)
+        assert bool((torch.isfinite(got) == fine).all()), b
+        assert bool((got[~fine & ~torch.isnan(want)] == want[~fine & ~torch.isnan(want)]).all())
+        assert bool(((got - want).abs() <= tol)[fine].all()), b
