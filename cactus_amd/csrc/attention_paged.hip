@@ -389,9 +389,12 @@ hipError_t launch_step(const PagedAttnArgs& a, const StepShape& s, hipStream_t s
 
 }  // namespace
 
-// The split rule.  A workgroup takes at least one block per wave (128 keys), and a batch is split until about 1024 workgroups
-// (four per CU) are there or nothing is left to split.
-StepShape step_shape(size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
+// The split rule.  Keys are split until as many workgroups are there as keep about 16 MB of cache requested, which is what the
+// memory's latency needs: 256 of four waves and two blocks each (one at head_dim 256), 512 at head_dim 64, whose blocks are half as
+// large.  More only make records: 4 sequences of 32k, 4 heads over 1 of 256: 18 us with 256, 29 with 1024; 4 of 32k, 32 heads over 8 of
+// 64: 37 and 28 with 512, 27 with 1024.  A round of a workgroup's waves takes 128 keys, and a split that saves fewer than three
+// rounds does not pay for the join (300 keys in 64 sequences, 16 heads over 8 of 128: 18 us in two splits, 10 in one).
+StepShape step_shape(size_t head_dim, size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
                      bool one_row_each) {
     StepShape s;
     const size_t group = q_heads / kv_heads;
@@ -401,8 +404,8 @@ StepShape step_shape(size_t batch, size_t max_context, size_t q_heads, size_t kv
     size_t keys = max_context;
     if (window && window + sink < keys) keys = window + sink;
     const size_t rounds = (keys + STEP_WAVES * STEP_KEYS - 1) / (STEP_WAVES * STEP_KEYS);
-    const size_t want = (1024 + items - 1) / items;
-    s.splits = (int)(rounds < 1 ? 1 : rounds < want ? rounds : want);
+    const size_t fill = head_dim == 64 ? 512 : 256, want = items >= fill ? 1 : fill / items, most = rounds < want ? rounds : want;
+    s.splits = most > 1 && rounds - (rounds + most - 1) / most >= 3 ? (int)most : 1;
     return s;
 }
 

@@ -69,7 +69,7 @@ struct PagedAttnArgs {
 struct StepShape {
     int row_tiles, rows, splits;
 };
-StepShape step_shape(size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
+StepShape step_shape(size_t head_dim, size_t batch, size_t max_context, size_t q_heads, size_t kv_heads, size_t window, size_t sink,
                      bool one_row_each);
 hipError_t launch_attention_step(int head_dim, const PagedAttnArgs& a, const StepShape& s, hipStream_t st);
 // attention_tiles.hip: 128 rows at a time, over the pages or over FP16 rows.  blocks: workgroups, records: split records, joined:

@@ -115,7 +115,7 @@ PagedPlan paged_plan(const cactus_hip_paged_kv& c, size_t batch, size_t tokens, 
     p.by_step = one_row_each || tokens * (q_heads / c.kv_heads) < 64 * batch;
     p.by_tile = !one_row_each;
     if (p.by_step) {
-        p.step = step_shape(batch, max_context, q_heads, c.kv_heads, window, sink, one_row_each);
+        p.step = step_shape(c.head_dim, batch, max_context, q_heads, c.kv_heads, window, sink, one_row_each);
         p.step_items = batch * c.kv_heads * p.step.row_tiles * p.step.splits;
         if (p.step.splits > 1) p.step_bytes = p.step_items * p.step.rows * (c.head_dim + 2) * sizeof(float);
     }
