@@ -176,6 +176,7 @@ __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int
     };
     int count = 0;
     for (int i = 0; i < per; i++) count += tiles_of(lane * per + i);
+    count = min(count, 1 << 23);         // offsets that are none can count rows many times over: no sum of these passes an int
     const int upto = sum_upto(count), tiles = __builtin_amdgcn_readlane(upto, 63), pairs = min(tiles, resident(D)) * a.kv_heads;
     p.splits = min(max(resident(D) / max(pairs, 1), 1), most);
     p.id = JOIN ? block : block / p.splits;
