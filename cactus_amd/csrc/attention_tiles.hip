@@ -742,10 +742,14 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 }  // namespace
 
 // A tile kernel's launch: a slot per tile of a sequence's rows and kv head, and key splits where that leaves most of the chip
-// idle, each of at least 512 keys.  Up to COUNTED sequences the kernel chooses the splits (place_of): more than one only while
-// they are all resident, so that at most half as many row tiles x heads are joined.
+// idle, each of at least 128 keys, at head_dim 64, whose tiles are quick beside the join, 256 (256 rows on 344 keys, 16 heads over 8 of
+// 128: 18.0 us with 128, 20.4 with 256, 22.7 with 512 at least; 4 heads over 1 of 256: 17, 23, 32; 4 x 100 rows on 900 keys, 32 heads
+// over 8 of 64: 29.0, 29.5, 24.3, but 256 rows on 944 keys 26, 20, 25).  `beside` the step kernel, where most sequences and often
+// all are not its, 512: the join is a launch for all of them (63 single tokens on 1000 keys 27.8 us, with 128 keys at least 34.0).
+// Up to COUNTED sequences the kernel chooses the splits (place_of): more than one only while they are all resident, so that at
+// most half as many row tiles x heads are joined.
 TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
-                     size_t window, size_t sink) {
+                     size_t window, size_t sink, bool beside) {
     TileShape s;
     const size_t rows = tokens * (q_heads / kv_heads), size = tile_rows((int)head_dim), least = (rows + size - 1) / size;
     s.slots = (int)(batch == 1 ? least : rows / size + batch);                        // slot_begin
@@ -753,7 +757,7 @@ TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_co
     size_t keys = max_context;
     if (window && window + sink + size < keys) keys = window + sink + size;
     const bool counted = batch <= (size_t)COUNTED;
-    const size_t fill = resident((int)head_dim), most = keys / 512, want = fill / ((counted ? least : s.slots) * kv_heads);
+    const size_t fill = resident((int)head_dim), most = keys / (beside ? 512 : head_dim == 64 ? 256 : 128), want = fill / ((counted ? least : s.slots) * kv_heads);
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
     s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
     s.blocks = counted && s.splits > 1 ? (items > fill ? items : fill) : items * s.splits;
