@@ -16,11 +16,11 @@
 // as one fma per score.  Values take one v_pk_fma_f16 per two more, to b 2^-9 (exact): left with the offset the output would be
 // a small difference of large sums.
 // A page has one scale per head.  Its key scale multiplies the scores of 16 keys at once; its value scale is added to the
-// scores as a logarithm, so that weights (exp2(s + log2 s_v - running maximum), rounded to binary16 against the maximum
+// scores as a logarithm, so that weights (exp2(s + log2 s_v - running maximum + LIFT), rounded to binary16 against the maximum
 // of all of them) never leave binary16's range whatever the scales are, and the sum of the plain weights takes the
 // fp32 weights over s_v back.
 // The next block's rows are requested before the current one is computed (registers, two blocks deep).  The output is
-// rescaled only when a maximum has grown by more than 2^8.
+// rescaled only when a maximum has grown by more than 2^LAG.
 // Measured (16 heads over 8, D = 128): 256 sequences of 300 to 700 keys 50.1 us = 5.2 TB/s; 4 of 32k, 32 heads over 8, 45.8 us =
 // 5.6 TB/s and 4.6 for the join; one of 4096 5.8 + 3.4 us; 64 of window 508 + 4, 4 heads over 1, D = 256, 11.0 + 3.9 us.
 #include "paged.hip.h"
@@ -211,7 +211,7 @@ void attention_step_kernel(const PagedAttnArgs a, const int splits, const int ro
     const auto values = [&](StepBlock<D>& t) {
         float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
         top = rows_max(top);
-        if (__any(top > m + 8.0f)) {
+        if (__any(top > m + LAG)) {
             const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
             m = to;
             l *= f;
@@ -219,8 +219,9 @@ void attention_step_kernel(const PagedAttnArgs a, const int splits, const int ro
             for (int i = 0; i < DT; i++) o[i] *= f;
         }
         float w[8];
+        const float unit = m - LIFT;
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = __builtin_amdgcn_exp2f(s[e] - m);
+        for (int e = 0; e < 8; e++) w[e] = __builtin_amdgcn_exp2f(s[e] - unit);
         l = fmaf((w[0] + w[1]) + (w[2] + w[3]), inv_vs[0], l);
         l = fmaf((w[4] + w[5]) + (w[6] + w[7]), inv_vs[1], l);
         v8h p;

@@ -9,7 +9,7 @@
 //   O^T = V^T P^T V^T through the transposing LDS read (ds_read_b64_tr_b16); P is the lane's own scores, in the key order the
 //                 first product left them in (the contraction order is free)
 // so the softmax's maximum and sum are in-lane work plus one exchange with lane ^ 32, and weights never move.  The rest is the
-// online softmax in base 2; (l, O) move to a new maximum only when it has grown by more than 2^8.
+// online softmax in base 2; (l, O) move to a new maximum only when it has grown by more than 2^LAG.
 // Key tiles (64 keys, 32 at head_dim 256) are double-buffered: the next one's loads go out between the products of the scores (a
 // burst of them holds every wave up) and it is stored to the other buffer behind the output's products, one barrier per tile.
 // Loads past a sequence's last row are cut off by the buffer's length and give zeros, so no tile needs a branch.  16-byte chunks
@@ -17,7 +17,8 @@
 // meet on a bank.
 // INT8 pages become halves on the way into LDS: keys as the subnormal (b + 128) 2^-24 (one v_perm per two; the offset leaves
 // with the score's fma), values as b 2^-9.  Page scales enter as in attention_paged.hip.
-// Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count); everything else is fp32.
+// Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count, down to 2^-25 of the largest: LIFT); everything
+// else is fp32.
 //
 // Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 83 us, 825 TFLOP/s (a large FP16 matrix product reaches
 // 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 89 us, 475.  24 prompts of 17 to 300 tokens,
@@ -481,7 +482,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
                 for (int r = 0; r < AR; r += 2) top = fmaxf(fmaxf(s[t][r], s[t][r + 1]), top);
             top = row_max<RW>(top) * c0;
         }
-        if (__any(top > m + 8.0f)) {
+        if (__any(top > m + LAG)) {
             const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
             m = to;
             l *= f;
@@ -490,9 +491,10 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
 #pragma unroll
                 for (int r = 0; r < AR; r++) o[i][r] *= f;
         }
+        const float lift = LIFT - m;
         if constexpr (PAGED) {
 #pragma unroll
-            for (int g = 0; g < GROUPS; g++) add[g] -= m;
+            for (int g = 0; g < GROUPS; g++) add[g] += lift;
         }
         // The wave that feeds the matrix cores goes before the one that is elsewhere in its tile: 2% at D = 128, nothing at 256; at
         // 64, where the products are short against the rest, it costs 4%.
@@ -505,7 +507,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
                 const int quad = 2 * f + half, t = quad / (AR / 4), r0 = quad % (AR / 4) * 4;
                 float w[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(PAGED ? fmaf(s[t][r0 + e], up[group_of(t, r0)], add[group_of(t, r0)]) : fmaf(s[t][r0 + e], c0, -m));
+                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(PAGED ? fmaf(s[t][r0 + e], up[group_of(t, r0)], add[group_of(t, r0)]) : fmaf(s[t][r0 + e], c0, lift));
                 const float sum = (w[0] + w[1]) + (w[2] + w[3]);
                 l = PAGED ? fmaf(sum, inv_vs[group_of(t, r0)], l) : l + sum;
 #pragma unroll

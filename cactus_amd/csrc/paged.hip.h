@@ -6,6 +6,13 @@
 
 namespace cactus_hip {
 
+// Softmax weights are rounded to binary16 before they meet the values.  They are held as exp2(score - maximum + LIFT) against a
+// maximum that may be up to LAG behind (the output is rescaled only when it has fallen further behind), so the largest is
+// 2^(LAG + LIFT) at most and binary16's full 2^-11 reaches down to 2^-25 of the largest weight, a step of 2^-35 below that.
+// Without the lift, weights of 2^-24 of the largest were a single step, and 8000 of them beside a first token that takes
+// nearly everything were off by half.  The factor leaves with the division by their sum.
+constexpr float LAG = 4.0f, LIFT = 11.0f;
+
 struct Rows {
     int first, count;
 };

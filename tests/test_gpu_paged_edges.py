@@ -1,0 +1,95 @@
+"""GPU tests of the paged cache's operators (cactus_amd/paged.py) where numbers are small, infinite or not numbers: weights far
+below the largest, infinite values that are seen, page scales that no append makes, codes that are requantized many times."""
+import math
+
+import pytest
+
+from tests import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def P():
+    import cactus_amd.hip as hip
+    import cactus_amd.paged as paged
+    hip.init(0)
+    return paged
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+# ------------------------------------------------------------------------------------- weights far below the largest
+
+# A weight is rounded to binary16 after it was raised by 2^11 against a maximum that is at most 2^4 behind, so it is off by half a
+# step, 2^-11 of itself, or 2^-25 of the raised unit: 2^-36 of the largest weight.
+SMALLEST = 2.0 ** -36
+
+
+def first_key_and_the_rest(bits, keys):
+    """exp2 weights: 1 for key 0, whose value is zero, and 2^-bits for each of the others, whose values are one."""
+    w = 2.0 ** -bits
+    total = 1 + (keys - 1) * w
+    want = (keys - 1) * w / total
+    # the weights' rounding; scores (one product of small numbers each) and their base-2 argument in fp32: 4 roundings of `bits`; the
+    # sums' over the keys; the output's own
+    tol = (keys - 1) * (max(w * R.U16, SMALLEST) + w * (4 * bits * R.U32 + keys * R.U32)) / total + want * R.U16 + 2.0 ** -25
+    return want, tol
+
+
+@pytest.mark.parametrize("bits", [10, 14.25, 17.5, 20, 21.75, 23.5, 24.5, 25.25, 26.5])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_small_weights_beside_a_large_one(P, D, bits):
+    """What a first token without a value of its own does: it takes nearly all of the weight and the others share the rest."""
+    n, page, scale = 8192, 64, math.log(2)
+    want, tol = first_key_and_the_rest(bits, n)
+    q, k, v = (torch.zeros((n, 1, D), dtype=torch.float16, device="cuda") for _ in range(3))
+    q[:, 0, 0] = 1.0
+    k[0, 0, 0] = bits
+    v[1:] = 1.0
+    out = P.attention_ragged(q, k, v, i32([0, n]).cuda(), scale=scale)[-1].cpu().double()
+    assert bool(((out - want).abs() <= tol).all()), float(out[0, 0] / want - 1)
+    kv = P.empty_pages(n // page, 1, D, page)
+    kv[0].view(-1, D)[0, 0] = int(4 * bits)
+    kv[1].view(-1, D)[1:] = 64
+    kv[2].fill_(0.25)
+    kv[3].fill_(1 / 64)
+    t = torch.arange(n // page, dtype=torch.int32, device="cuda")[None]
+    one = P.attention(q[:1], kv, t, i32([n]).cuda(), scale=scale)[-1].cpu().double()
+    many = P.attention(q[:70], kv, t, i32([n]).cuda(), cu_seqlens=i32([0, 70]).cuda(), scale=scale)[-1].cpu().double()
+    # over pages the weights of a launch's key splits are raised against each split's own maximum, which only helps
+    assert bool(((one - want).abs() <= tol).all()), float(one[0, 0] / want - 1)
+    assert bool(((many - want).abs() <= tol).all()), float(many[0, 0] / want - 1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("step", [0.5, 3.0, 5.0])
+def test_a_maximum_that_grows_with_every_key(P, D, step):
+    """Scores that rise from key to key: the running maximum moves all the time, by less and by more than it may be behind."""
+    n, page, scale = 700, 16, math.log(2)
+    top = 127 * 0.25                                     # of the scores, as codes of scale 1/4 can hold them
+    codes = torch.arange(n).float().mul(4 * step).sub(4 * step * (n - 1)).add(4 * top).clamp_min(-508).div(4).round()
+    k = torch.zeros((n, 1, D), dtype=torch.float16)
+    k[:, 0, 0] = codes * 0.25
+    v = torch.randint(-127, 128, (n, 1, D), generator=torch.Generator().manual_seed(D)).half() / 64
+    q = torch.zeros((n, 1, D), dtype=torch.float16)
+    q[:, 0, 0] = 4.0
+    rows = torch.tensor([0, 1, 15, 16, 63, 64, 65, 300, 511, n - 1])
+    want, tol = R.attend(q[rows], k, v, rows, 0, 0, scale)
+    out = P.attention_ragged(q.cuda(), k.cuda(), v.cuda(), i32([0, n]).cuda(), scale=scale).cpu().double()
+    assert bool(((out[rows] - want).abs() <= tol).all())
+    kv = [x.cuda() for x in P.empty_pages((n + page - 1) // page, 1, D, page)]
+    flat = lambda x: torch.cat([x[:, 0], x.new_zeros((-n % page, D))]).view(-1, 1, page, D).to(torch.int8).cuda()  # noqa: E731
+    kv[0].copy_(flat(k.float() * 4))
+    kv[1].copy_(flat(v.float() * 64))
+    kv[2].fill_(0.25)
+    kv[3].fill_(1 / 64)
+    t = torch.arange(kv[0].shape[0], dtype=torch.int32, device="cuda")[None]
+    for m in (1, 60):
+        cu = None if m == 1 else i32([0, m]).cuda()
+        got = P.attention(q[:m].cuda(), kv, t, i32([n]).cuda(), cu_seqlens=cu, scale=scale)[-1:].cpu().double()
+        assert bool(((got - want[-1:]).abs() <= tol[-1:]).all()), m
