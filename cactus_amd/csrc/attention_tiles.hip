@@ -20,9 +20,9 @@
 // Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count, down to 2^-25 of the largest: LIFT); everything
 // else is fp32.
 //
-// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 83 us, 825 TFLOP/s (a large FP16 matrix product reaches
-// 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 89 us, 475.  24 prompts of 17 to 300 tokens,
-// D = 64: 18.2 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 43 us, 8 of them the join's.
+// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 83 us, 829 TFLOP/s (a large FP16 matrix product reaches
+// 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 87 us, 485.  24 prompts of 17 to 300 tokens,
+// D = 64: 17.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 43 us, 8 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"
@@ -48,7 +48,6 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
-typedef unsigned short v8u __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
 template <int RW>
@@ -211,16 +210,16 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
     // INT8, per 16-key group: factor of the score, (unused), log2 of the value scale, its reciprocal.  A group without a page has the
     // logarithm -inf, which is all the masking it needs.  The factor is above zero, so that a masked score stays -inf.
     __shared__ __attribute__((aligned(16))) float s_scales[NG][2][GROUPS][4];
-    // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  s_odd: 1 + the
-    // tile, not seen whole by every row, that holds such values; s_marks: +inf, -inf, NaN bits of every row's dims
-    __shared__ int s_odds[NG][2], s_marked;
+    // FP16 rows: a value that is not finite must not reach a row that does not see its key, and 0 * inf is NaN.  So tiles that some
+    // row does not see whole get zeros in their place (s_odd: there were any), and where they belong is looked up at the end.
+    // s_marks: +inf, -inf, NaN bits of every row's dims
+    __shared__ int s_odd;
     __shared__ uint32_t s_marks[PAGED ? 1 : 3][PAGED ? 1 : TILE_ROWS][D / 32];
 
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // in the group
     const int grp = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int n = lane % RW, h = lane / RW;
     float(*const s_scale)[GROUPS][4] = s_scales[grp];
-    int* const s_odd = s_odds[grp];
     const int group = a.q_heads / a.kv_heads;
     const Place at = place_of<D, false>(a, blockIdx.x, most_splits, slots, group);
     const int tile = at.tile, b = at.b, splits = PAGED ? at.splits : 1, split = PAGED ? at.split : 0, head = at.id % a.kv_heads;
@@ -340,7 +339,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
 #pragma unroll
                     for (int e = 0; e < 4; e++) odd |= (((uint32_t)t.v[i][e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
                 if (odd) {
-                    s_odd[buf] = u + 1;
+                    s_odd = 1;
 #pragma unroll
                     for (int i = 0; i < Load::PIECES; i++)
 #pragma unroll
@@ -532,37 +531,6 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
             if (i < PRODUCTS - NDT) __builtin_amdgcn_sched_group_barrier(0x402, SHARE, 1);
         }
         if constexpr (D > 64) __builtin_amdgcn_s_setprio(0);
-        if constexpr (!PAGED) {
-            if (s_odd[buf] == u + 1) {
-                // The values that are not finite are zero in LDS (stash).  Every row that puts weight on such a key is marked:
-                // the output of that dim becomes what adding the value makes of it.
-                uint32_t mine = 0;
-#pragma unroll
-                for (int f = 0; f < FRAGS; f++) {
-                    v4i bits = __builtin_bit_cast(v4i, p[f]);
-                    asm volatile("" : "+v"(bits));       // not before the branch: without this every tile pays for it
-                    const v8u w = __builtin_bit_cast(v8u, bits);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) mine = 2 * mine + (w[e] ? 1u : 0u);       // bit 8 FRAGS - 1 - (8 f + e)
-                }
-                s_marked = 1;
-#pragma unroll 1
-                for (int k = 0; k < BK && key + k <= last; k++) {
-                    const int in = k % FK, bit = 8 * FRAGS - 1 - (8 * (k / FK) + 4 * (in / QUAD) + (k & 3));
-                    const bool weighed = ((__shfl(mine, n + RW * (in % QUAD / 4)) >> bit) & 1) != 0;
-#pragma unroll 1
-                    for (int d0 = 0; d0 < D; d0 += 64) {
-                        const uint32_t x = a.v[(size_t)(rows.first + key + k) * a.v_stride + (size_t)head * D + d0 + lane];
-                        for (unsigned long long odd = __ballot((x & 0x7c00u) == 0x7c00u); odd; odd &= odd - 1) {
-                            const int at = __builtin_ctzll(odd), d = d0 + at;
-                            const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)x, at);
-                            const int kind = y == 0x7c00u ? 0 : y == 0xfc00u ? 1 : 2;
-                            if (weighed) atomicOr(&s_marks[kind][wave * RW + n][d >> 5], 1u << (d & 31));
-                        }
-                    }
-                }
-            }
-        }
     };
 
     if (u0 < u1) {
@@ -575,9 +543,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
         if (first < u1) fetch(t, first);
         look_up(first + NG);
         if constexpr (!PAGED) {
-            if (tid < 2) s_odd[tid] = 0;
-            if (threadIdx.x == 0) s_marked = 0;
-            for (int i = threadIdx.x; i < 3 * TILE_ROWS * (D / 32); i += 256 * NG) (&s_marks[0][0][0])[i] = 0;
+            if (threadIdx.x == 0) s_odd = 0;
             __syncthreads();
         }
         if (first < u1) stash(zero, t, first);
@@ -629,6 +595,66 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
                 for (int e = 0; e < 4; e++) o[i][r + e] = fmaf(x[e], f1, o[i][r + e] * f0);
             }
     }
+    if constexpr (!PAGED) {
+        // Values that are not finite, once more.  In tiles that all rows see whole they have gone through the products: such a dim is
+        // not finite, but what it is depends on roundings (weights of 0 in binary16, rescaling by 0 make NaN of an infinity).  In the
+        // others they were left out.  If there are any of either kind, the wave looks through the values that its rows see, 4 KB at a
+        // time, and every row that sees one has it in that dim, whatever it weighs.
+        float zero = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NDT; i++)
+#pragma unroll
+            for (int r = 0; r < AR; r++) zero = fmaf(o[i][r], 0.0f, zero);
+        if (__any(zero != zero || s_odd != 0)) {
+            constexpr int CHUNKS_ROW = D / 8, KEYS = 64 / CHUNKS_ROW, LOADS = 4, KIND = TILE_ROWS * (D / 32);
+            uint32_t* const marks = &s_marks[0][wave * RW][0];
+#pragma unroll 1
+            for (int i = lane; i < RW * (D / 32); i += 64)
+                for (int kind = 0; kind < 3; kind++) marks[kind * KIND + i] = 0;
+            const auto scan = [&](int from, int to) {
+#pragma unroll 1
+                for (int key0 = from; key0 < to; key0 += LOADS * KEYS) {
+                    v4i x[LOADS];            // keys past the last are the last one again
+#pragma unroll
+                    for (int j = 0; j < LOADS; j++) {
+                        const int key = min(key0 + j * KEYS + lane / CHUNKS_ROW, to - 1);
+                        x[j] = *reinterpret_cast<const v4i*>(a.v + (size_t)(rows.first + key) * a.v_stride + (size_t)head * D + lane % CHUNKS_ROW * 8);
+                    }
+#pragma unroll
+                    for (int j = 0; j < LOADS; j++) {
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) odd |= (((uint32_t)x[j][e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                        for (unsigned long long who = __ballot(odd != 0); who; who &= who - 1) {
+                            const int src = __builtin_ctzll(who), key = min(key0 + j * KEYS + src / CHUNKS_ROW, to - 1), d0 = src % CHUNKS_ROW * 8;
+                            const bool sees = key <= pos && (!a.window || pos - key <= a.window || key < a.sink);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const uint32_t y = ((uint32_t)__builtin_amdgcn_readlane(x[j][e >> 1], src) >> (16 * (e & 1))) & 0xffffu;
+                                if ((y & 0x7c00u) != 0x7c00u) continue;
+                                const int kind = y == 0x7c00u ? 0 : y == 0xfc00u ? 1 : 2;
+                                if (sees && h == 0) atomicOr(&marks[kind * KIND + n * (D / 32) + ((d0 + e) >> 5)], 1u << ((d0 + e) & 31));
+                            }
+                        }
+                    }
+                }
+            };
+            const int low = a.window ? max(wpos_first - a.window, 0) : 0;
+            scan(0, min(a.window ? a.sink : 0, low));
+            scan(low, wpos_last + 1);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");      // the rows' marks are the wave's own
+#pragma unroll
+            for (int i = 0; i < NDT; i++)
+#pragma unroll
+                for (int r = 0; r < AR; r++) {
+                    const int d = RW * i + QUAD * (r >> 2) + (r & 3);           // and 4 h, which stays inside the word
+                    const uint32_t* at = marks + n * (D / 32) + (d >> 5);
+                    const int bit = (d & 31) + 4 * h;
+                    const bool plus = (at[0] >> bit) & 1, minus = (at[KIND] >> bit) & 1, none = (at[2 * KIND] >> bit) & 1;
+                    o[i][r] = none || (plus && minus) ? NAN : plus ? INFINITY : minus ? -INFINITY : o[i][r];
+                }
+        }
+    }
     if (wave * RW + n >= R) return;
     const float unit = PAGED ? 512.0f : 1.0f;
     if (splits > 1) {
@@ -649,21 +675,6 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
             }
     } else {
         const float inv = l > 0.0f || l != l ? unit / l : 0.0f;
-        if constexpr (!PAGED) {
-            if (s_marked) {
-#pragma unroll 1
-                for (int kind = 0; kind < 3; kind++) {
-                    const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-#pragma unroll
-                    for (int i = 0; i < NDT; i++)
-#pragma unroll
-                        for (int r = 0; r < AR; r++) {
-                            const int d = RW * i + QUAD * (r >> 2) + (r & 3);      // and 4 h, which stays inside the word
-                            o[i][r] += (s_marks[kind][wave * RW + n][d >> 5] >> ((d & 31) + 4 * h)) & 1 ? add : 0.0f;
-                        }
-                }
-            }
-        }
         uint16_t* out = a.out + ((size_t)token * a.q_heads + qh) * D + 4 * h;
 #pragma unroll
         for (int i = 0; i < NDT; i++)

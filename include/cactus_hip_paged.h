@@ -81,8 +81,9 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
                                        size_t workspace_bytes, void* stream);
 
 /* FP16 attention of whole prompts, causal, packed by cu_seqlens (required); row i of a sequence stands at position i.  A
- * key or value row that a query does not see has no influence on it whatever it holds (infinities and NaN included).  One
- * that it sees with less than 2^-36 of its largest weight may count as not seen in this. */
+ * key or value row that a query does not see has no influence on it whatever it holds (infinities and NaN included).  A
+ * value that it sees and that is not finite is in its output whatever it weighs: an infinity as that infinity, two of different
+ * sign and a NaN as NaN. */
 int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride, const cactus_half_t* k, size_t k_stride,
                                         const cactus_half_t* v, size_t v_stride, cactus_half_t* output,
                                         const int32_t* cu_seqlens, size_t batch, size_t tokens, size_t num_q_heads,

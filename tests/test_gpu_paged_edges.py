@@ -93,3 +93,62 @@ def test_a_maximum_that_grows_with_every_key(P, D, step):
         cu = None if m == 1 else i32([0, m]).cuda()
         got = P.attention(q[:m].cuda(), kv, t, i32([n]).cuda(), cu_seqlens=cu, scale=scale)[-1:].cpu().double()
         assert bool(((got - want[-1:]).abs() <= tol[-1:]).all()), m
+
+
+# ------------------------------------------------------------------------------------------- infinite values that are seen
+
+def check_infinities(P, D, H, lengths, window, sink, rows, heads):
+    """Values that are not finite in tiles that rows see whole and in those they do not, on keys that weigh next to nothing (about
+    2^-46 at head_dim 64, 2^-92 at 256) beside the first key of a sequence, or beside a later one that outgrows what came before."""
+    gen = torch.Generator().manual_seed(D + window)
+    T, n, base = sum(lengths), lengths[-1], sum(lengths[:-1])
+    q = torch.ones((T, H, D), dtype=torch.float16)
+    k = (torch.randn((T, H, D), generator=gen) / 16).half()
+    v = torch.randn((T, H, D), generator=gen).half()
+    k[base] = 4.0
+    k[base + n // 2] = 8.0
+    for key, dim, x in ((1, 0, math.inf), (20, 7, math.inf), (33, 7, math.inf), (70, 8, -math.inf), (5, 9, math.inf), (140, 9, -math.inf),
+                        (64, D - 1, math.nan), (n - 40, 40, -math.inf), (n - 1, 41, math.inf), (n - 2, 42, math.nan)):
+        v[base + key, :, dim] = x
+    cu = R.offsets(lengths)
+    out = P.attention_ragged(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), window=window, sink=sink).cpu().double()
+    assert bool(torch.isfinite(out[:base]).all())
+    at = torch.tensor(rows)
+    for h in heads:
+        one = slice(h, h + 1)
+        want, tol = R.attend(q[base + at, one], k[base:, one], v[base:, one], at, window, sink)
+        got, fine = out[base + at, one], torch.isfinite(want)
+        assert not bool(fine.all())
+        assert bool((torch.isnan(got) == torch.isnan(want)).all())
+        whole = ~torch.isnan(want) & ~fine
+        assert bool((got[whole] == want[whole]).all())
+        assert bool(((got - want).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window,sink", [(0, 0), (90, 0), (100, 6), (150, 70)])
+def test_infinite_values_on_keys_of_no_weight(P, D, window, sink):
+    n = 330
+    rows = [0, 1, 5, 19, 20, 21, 33, 63, 64, 69, 70, 100, 110, 127, 128, 140, 141, 164, 165, 166, 200, 255, 256, 289, 290, 291, 328, 329]
+    check_infinities(P, D, 2, [37, n], window, sink, rows, [0, 1])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sink", [(0, 0), (300, 6)])
+def test_infinite_values_where_one_group_takes_all_keys(P, D, window, sink):
+    check_infinities(P, D, 40, [300, 1400], window, sink, [0, 20, 69, 140, 320, 321, 641, 699, 700, 1000, 1359, 1360, 1399], [0, 39])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_infinite_values_behind_a_query_that_is_not_a_number(P, D):
+    """The row of such a query is not a number in any dim, its neighbours are what they would be without it."""
+    gen = torch.Generator().manual_seed(D)
+    n = 200
+    q, k, v = (torch.randn((n, 1, D), generator=gen).half().cuda() for _ in range(3))
+    v[3, 0, 5] = math.inf
+    want = P.attention_ragged(q, k, v, i32([0, n]).cuda())
+    q[150, 0, 9] = math.nan
+    got = P.attention_ragged(q, k, v, i32([0, n]).cuda())
+    assert bool(torch.isnan(got[150]).all())
+    want[150] = got[150] = 0
+    assert torch.equal(got, want) and bool((got[3:150, 0, 5] == math.inf).all()) and bool(torch.isfinite(got[:3]).all())
