@@ -192,7 +192,7 @@ void attention_step_kernel(const PagedAttnArgs a, const int splits, const int ro
                                                              q[2 * i + 1], acc, 0, 0, 0);
             }
             // scale * log2 e * s_k * (2^24 acc - 128 sum q) + log2 s_v
-            const float vs = fmaxf(t.vs[h], 1e-20f), c = c0 * t.ks[h], up = c * 16777216.0f, add = fmaf(c, bias, __log2f(vs));
+            const float vs = fmaxf(page_scale(t.vs[h]), 1e-20f), c = c0 * page_scale(t.ks[h]), up = c * 16777216.0f, add = fmaf(c, bias, __log2f(vs));
             inv_vs[h] = 1.0f / vs;
 #pragma unroll
             for (int r = 0; r < 4; r++) s[4 * h + r] = fmaf(acc[r], up, add);

@@ -377,7 +377,7 @@ void attention_tile_kernel(const PagedAttnArgs a, const int most_splits, const i
             }
         }
         if (PAGED && tid < 2 * GROUPS) {         // worked out once here, not by every wave
-            const float x = t.page < 0 ? 0.0f : fmaxf(t.scale, 0.0f), v = fmaxf(x, 1e-20f);
+            const float x = t.page < 0 ? 0.0f : page_scale(t.scale), v = fmaxf(x, 1e-20f);
             const v2f two = tid & 1 ? v2f{t.page < 0 ? -INFINITY : __log2f(v), t.page < 0 ? 0.0f : __builtin_amdgcn_rcpf(v)}
                                     : v2f{fmaxf(x * c0 * 16777216.0f, 1e-30f), 0.0f};
             *reinterpret_cast<v2f*>(&s_scale[buf][tid >> 1][2 * (tid & 1)]) = two;

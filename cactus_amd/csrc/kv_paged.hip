@@ -195,7 +195,7 @@ __global__ __launch_bounds__(1024) void append_paged_kernel(const PagedAppendArg
         const int kv_head = value ? item - a.c.kv_heads : item;
         const size_t ph = (size_t)page * a.c.kv_heads + kv_head;
         float* scale = (value ? a.c.vs : a.c.ks) + ph;
-        const float old = on && e_lo > 0 ? *scale : 0.0f;
+        const float old = on && e_lo > 0 ? page_scale(*scale) : 0.0f;
         if constexpr (!STEP) {
             for (int i = tid; i < HP; i += blockDim.x) s_max[i] = 0;
             __syncthreads();
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void read_paged_kernel(const PagedReadArgs a) 
         uint16_t* out = (which ? a.v_out : a.k_out) + ((size_t)row * a.c.kv_heads + h) * D + d;
         v8h lo{}, hi{};
         if (page >= 0) {
-            const float s = (which ? a.c.vs : a.c.ks)[ph];
+            const float s = page_scale((which ? a.c.vs : a.c.ks)[ph]);
             const v4i q = *reinterpret_cast<const v4i*>((which ? a.c.v : a.c.k) + src);
 #pragma unroll
             for (int e = 0; e < 8; e++) {

@@ -1,6 +1,8 @@
 // Device helpers shared by the kernels of the paged cache: packed rows, their owners, pages.
 #pragma once
 
+#include <math.h>
+
 #include "common.hip.h"
 #include "paged.h"
 
@@ -56,6 +58,9 @@ __device__ __forceinline__ int page_of(const PagedCache& c, int b, int i) {
     const int p = c.tables[(size_t)b * c.table_width + i];
     return p >= 0 && p < c.num_pages ? p : -1;
 }
+
+// A page's scale as every kernel takes it: what is not positive and finite (append makes no such scale) is zero.
+__device__ __forceinline__ float page_scale(float s) { return s > 0.0f && s < INFINITY ? s : 0.0f; }
 
 // Tokens of sequence b that its table can hold.  The lengths are device data that nobody checked: between 0 and 2^30, positions
 // and their differences stay in an int.

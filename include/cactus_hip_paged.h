@@ -6,7 +6,8 @@
  * holds ONE scale per kv head for its keys and one for its values:
  *
  *   k, v            int8  [num_pages][kv_heads][page_size][head_dim]      (page, head): one contiguous run
- *   k_scales, ...   float [num_pages][kv_heads]                           value = int8 * scale
+ *   k_scales, ...   float [num_pages][kv_heads]                           value = int8 * scale; a scale that
+ *                                                         is not positive and finite counts as zero
  *   block_tables    int32 [batch][table_width]    page of tokens page_size * i .. of sequence b in entry [b][i]
  *
  * page_size is 16, 32, 64 or 128 and head_dim 64, 128 or 256; all buffers are 16-byte aligned device memory.  The pages a

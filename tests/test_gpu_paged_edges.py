@@ -152,3 +152,31 @@ def test_infinite_values_behind_a_query_that_is_not_a_number(P, D):
     assert bool(torch.isnan(got[150]).all())
     want[150] = got[150] = 0
     assert torch.equal(got, want) and bool((got[3:150, 0, 5] == math.inf).all()) and bool(torch.isfinite(got[:3]).all())
+
+
+# ------------------------------------------------------------------------------------------- page scales that are none
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [-0.02, -0.0, math.nan, math.inf, -math.inf])
+def test_a_scale_that_is_not_positive_and_finite_counts_as_zero(P, D, which, bad):
+    """In every call alike: one row, many rows, tokens read back, tokens appended behind such ones."""
+    gen = torch.Generator().manual_seed(D)
+    page, H, n = 16, 2, 75
+    kv = [torch.randint(-127, 128, (5, H, page, D), generator=gen, dtype=torch.int8).cuda() for _ in range(2)]
+    kv += [(0.01 + 0.02 * torch.rand((5, H), generator=gen)).cuda() for _ in range(2)]
+    q = torch.randn((40, 4, D), generator=gen).half().cuda()
+    rows = torch.randn((3, H, D), generator=gen).half().cuda()
+    t, ctx = i32([[3, 1, 0, 2, 4]]).cuda(), i32([n]).cuda()
+
+    def results(value):
+        x = [y.clone() for y in kv]
+        x[2 if which == "k" else 3][[1, 4]] = value
+        out = [P.attention(q[39:], x, t, ctx), P.attention(q, x, t, ctx, cu_seqlens=i32([0, 40]).cuda()),
+               P.attention(q[:3], x, t, ctx, cu_seqlens=i32([0, 3]).cuda())]
+        out += P.kv_read(x, t, i32([0]).cuda(), i32([0, n]).cuda(), n)
+        P.kv_append(rows, rows, x, t, i32([n]).cuda(), 1e4, cu_seqlens=i32([0, 3]).cuda())
+        return out + [y[4] for y in x]
+
+    for a, b in zip(results(bad), results(0.0)):
+        assert bool(torch.isfinite(a).all()) and bool((a == b).all())
