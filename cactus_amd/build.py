@@ -40,6 +40,25 @@ def _stale(target, deps):
     return any(os.path.exists(d) and os.path.getmtime(d) > mt for d in deps)
 
 
+def _command_of(target):
+    """The command line that made a target, kept beside it: other flags make another object, whatever the dates say."""
+    try:
+        with open(target + ".cmd") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _forget(target):
+    if os.path.exists(target + ".cmd"):
+        os.remove(target + ".cmd")
+
+
+def _keep(target, cmd):
+    with open(target + ".cmd", "w") as f:
+        f.write(" ".join(cmd))
+
+
 def build(force=False, verbose=False):
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(HERE, "build")
@@ -52,14 +71,20 @@ def build(force=False, verbose=False):
         src = os.path.join(CSRC, s)
         obj = os.path.join(objdir, s + ".o")
         objs.append(obj)
-        if force or _stale(obj, [src] + hdrs):
-            cmd = ["hipcc"] + FLAGS + EXTRA_FLAGS.get(s, []) + (["-x", "hip"] if s.endswith(".cpp") else []) + ["-c", src, "-o", obj]
+        cmd = ["hipcc"] + FLAGS + EXTRA_FLAGS.get(s, []) + (["-x", "hip"] if s.endswith(".cpp") else []) + ["-c", src, "-o", obj]
+        if force or _stale(obj, [src] + hdrs) or _command_of(obj) != " ".join(cmd):
             if verbose:
                 print(" ".join(cmd))
-            procs.append((s, subprocess.Popen(cmd)))
-    for s, p in procs:
+            _forget(obj)             # until it is made: a compiler that was stopped half way leaves no object that counts
+            procs.append((s, obj, cmd, subprocess.Popen(cmd)))
+    failed = []
+    for s, obj, cmd, p in procs:
         if p.wait() != 0:
-            raise RuntimeError(f"hipcc failed on {s}")
+            failed.append(s)
+        else:
+            _keep(obj, cmd)
+    if failed:
+        raise RuntimeError(f"hipcc failed on {', '.join(failed)}")
     if force or procs or _stale(SO, objs):
         cmd = ["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", SO] + objs + ["-ldl"]
         if verbose:
