@@ -89,3 +89,15 @@ def test_a_failed_build_is_not_taken_for_a_built_one(builder, monkeypatch):
     builder.failing.clear()
     assert "b.cpp.o" in builder.built()
     assert builder.built() == []
+
+
+def test_the_entry_compiles_every_source_each_time(tmp_path, monkeypatch):
+    import __graft_entry__ as entry
+    (tmp_path / "cactus_amd").mkdir()
+    note = tmp_path / "called"
+    (tmp_path / "cactus_amd" / "build.py").write_text(
+        f"def build(force=False, verbose=False):\n    open({str(note)!r}, 'a').write('all ' if force else 'some ')\n")
+    monkeypatch.setattr(entry, "ROOT", str(tmp_path))
+    entry.build()
+    entry.build()
+    assert note.read_text() == "all all "
