@@ -157,9 +157,9 @@ int cactus_hip_kv_append_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
                                        size_t num_q_heads, const cactus_half_t* q_weight, const cactus_half_t* k_weight,
                                        float eps, float theta, void* stream) {
     const char* who = "kv_append_paged";
+    REFUSE_IF(bad_batch(cu_seqlens, batch, tokens));
     if (batch == 0 || tokens == 0) return CACTUS_HIP_OK;
     REFUSE_IF(bad_cache(cache, block_tables, table_width));
-    REFUSE_IF(bad_batch(cu_seqlens, batch, tokens));
     if (!positions) return refuse(who, "null positions");
     REFUSE_IF(bad_rows(k, k_stride, cache->kv_heads, cache->head_dim));
     REFUSE_IF(bad_rows(v, v_stride, cache->kv_heads, cache->head_dim));
@@ -223,9 +223,9 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
                                        size_t num_q_heads, float scale, size_t window, size_t sink, void* workspace,
                                        size_t workspace_bytes, void* stream) {
     const char* who = "attention_paged";
+    REFUSE_IF(bad_batch(cu_seqlens, batch, tokens));
     if (batch == 0 || tokens == 0) return CACTUS_HIP_OK;
     REFUSE_IF(bad_cache(cache, block_tables, table_width));
-    REFUSE_IF(bad_batch(cu_seqlens, batch, tokens));
     REFUSE_IF(bad_groups(num_q_heads, cache->kv_heads));
     REFUSE_IF(bad_window(window, sink));
     if (tokens * (num_q_heads / cache->kv_heads) > MAX_ROWS * 8) return refuse(who, too_many);
