@@ -137,8 +137,8 @@ __device__ __forceinline__ int slot_of(int rank, int slots, int kv_heads) {
 // lane for every 64th part of the batch, and numbers them without gaps.  As many workgroups as the registers hold (resident) fill the
 // chip, and a few more cost a second round (three chunks with 80 row tiles x heads, D = 128, take 47.4 us in 6 splits = 480
 // workgroups, 50.2 in 5 and 62 in 7; at D = 64 768 take 54 us and 512 60, at 256 103 and 86), so the keys get the largest number of
-// splits that stays within them.  Above, slots lie as slot_begin has them and the host's `most` goes by the largest number of
-// tiles there can be.
+// splits that stays within them.  Above, slots lie as slot_begin has them, and there are more than the chip holds at once whatever the
+// lengths: keys are not split.
 constexpr int resident(int D) { return D == 64 ? 768 : 512; }       // three waves per SIMD, or two
 constexpr int COUNTED = 1024;
 struct Place {
@@ -160,9 +160,9 @@ __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, int block, int
     Place p;
     p.tile = -1;
     if (a.batch > COUNTED) {
-        p.splits = most;
-        p.id = JOIN ? block : block / most;
-        p.split = JOIN ? 0 : block % most;
+        p.splits = 1;
+        p.id = block;
+        p.split = 0;
         const auto begin = [&](int i) { return slot_begin(a.cu, i, a.tokens, group, size, 1); };
         const int slot = slot_of(p.id / a.kv_heads, slots, a.kv_heads);
         p.b = owner_of(slot, a.batch, begin);
@@ -769,13 +769,13 @@ TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_co
     const size_t items = (size_t)s.slots * kv_heads;
     size_t keys = max_context;
     if (window && window + sink + size < keys) keys = window + sink + size;
-    const bool counted = batch <= (size_t)COUNTED;
-    const size_t fill = resident((int)head_dim), most = keys / (beside ? 512 : head_dim == 64 ? 256 : 128), want = fill / ((counted ? least : s.slots) * kv_heads);
+    const size_t fill = resident((int)head_dim), most = keys / (beside ? 512 : head_dim == 64 ? 256 : 128);
+    const size_t want = batch <= (size_t)COUNTED ? fill / (least * kv_heads) : 1;
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
     s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
-    s.blocks = counted && s.splits > 1 ? (items > fill ? items : fill) : items * s.splits;
-    s.records = s.splits == 1 ? 0 : counted ? fill : s.blocks;
-    s.joined = counted && items > fill / 2 ? fill / 2 : items;
+    s.blocks = s.splits > 1 && items < fill ? fill : items;
+    s.records = s.splits > 1 ? fill : 0;
+    s.joined = items < fill / 2 ? items : fill / 2;
     return s;
 }
 size_t tile_record_floats(size_t head_dim) { return tile_rows((int)head_dim) * (head_dim + 2); }

@@ -1,7 +1,11 @@
-"""CPU tests of the paged cache's boundary: calls that are almost empty (the checks run on the host, before anything is enqueued)."""
+"""CPU tests of the paged cache's boundary: calls that are almost empty, workspaces (the host decides
+both before anything is enqueued)."""
+import ctypes as C
+
 import pytest
 
-from tests.test_paged_cpu import append, attend, read, ragged, refused
+import cactus_amd.hip as H
+from tests.test_paged_cpu import append, attend, cache, ragged, read, refused
 
 
 @pytest.mark.parametrize("call", [append, attend])
@@ -14,3 +18,13 @@ def test_without_offsets_rows_and_sequences_are_the_same_number_also_when_one_is
 def test_calls_without_sequences_or_rows_do_nothing():
     assert append(batch=0, tokens=0) == 0 and attend(batch=0, tokens=0) == 0
     assert read(batch=0) == 0 and read(rows=0) == 0 and ragged(batch=0) == 0 and ragged(tokens=0) == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("context", [0, 500, 1 << 20])
+def test_chunks_of_more_than_1024_sequences_need_no_workspace(dim, context):
+    """Their row tiles fill the chip without splitting keys (64 rows each: all of them the tile kernel's)."""
+    c = cache(head_dim=dim, kv_heads=1)
+    need = lambda batch: H.lib.cactus_hip_attention_paged_workspace_bytes(C.byref(c), batch, 64 * batch, context, 1, 0, 0, 0)  # noqa: E731
+    assert need(1025) == 0 and need(1 << 16) == 0
+    assert (need(3) > 0) == (context >= 500)
