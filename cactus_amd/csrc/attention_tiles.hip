@@ -742,8 +742,9 @@ __global__ __launch_bounds__(256) void attention_tile_join_kernel(const PagedAtt
 
 template <int D, bool PAGED>
 hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
-    if (D < 256 && s.groups == 2)
-        attention_tile_kernel<D, PAGED, D < 256 ? 2 : 1><<<dim3((unsigned)s.blocks), dim3(512), 0, st>>>(a, s.splits, s.slots);
+    constexpr int NG = D < 256 && !PAGED ? 2 : 1;            // the most groups that a launch may have
+    if (s.groups == 2 && NG == 2)
+        attention_tile_kernel<D, PAGED, NG><<<dim3((unsigned)s.blocks), dim3(256 * NG), 0, st>>>(a, s.splits, s.slots);
     else
         attention_tile_kernel<D, PAGED, 1><<<dim3((unsigned)s.blocks), dim3(256), 0, st>>>(a, s.splits, s.slots);
     hipError_t e = hipGetLastError();
@@ -759,9 +760,11 @@ hipError_t launch(const PagedAttnArgs& a, const TileShape& s, hipStream_t st) {
 // 128: 18.0 us with 128, 20.4 with 256, 22.7 with 512 at least; 4 heads over 1 of 256: 17, 23, 32; 4 x 100 rows on 900 keys, 32 heads
 // over 8 of 64: 29.0, 29.5, 24.3, but 256 rows on 944 keys 26, 20, 25).  `beside` the step kernel, where most sequences and often
 // all are not its, 512: the join is a launch for all of them (63 single tokens on 1000 keys 27.8 us, with 128 keys at least 34.0).
+// FP16 prompts are not split; few row tiles of them get two groups of waves instead (one prompt of 4096 tokens 106 -> 95 us), which
+// over pages cost more than two workgroups (50.4 against 53.2 us).
 // Up to COUNTED sequences the kernel chooses the splits (place_of): more than one only while they are all resident, so that at
 // most half as many row tiles x heads are joined.
-TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
+TileShape tile_shape(size_t head_dim, bool paged, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
                      size_t window, size_t sink, bool beside) {
     TileShape s;
     const size_t rows = tokens * (q_heads / kv_heads), size = tile_rows((int)head_dim), least = (rows + size - 1) / size;
@@ -770,9 +773,9 @@ TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_co
     size_t keys = max_context;
     if (window && window + sink + size < keys) keys = window + sink + size;
     const size_t fill = resident((int)head_dim), most = keys / (beside ? 512 : head_dim == 64 ? 256 : 128);
-    const size_t want = batch <= (size_t)COUNTED ? fill / (least * kv_heads) : 1;
+    const size_t want = paged && batch <= (size_t)COUNTED ? fill / (least * kv_heads) : 1;
     s.splits = (int)(most < 1 || want < 1 ? 1 : most < want ? most : want);
-    s.groups = head_dim < 256 && items <= 512 && max_context == 0 ? 2 : 1;
+    s.groups = !paged && head_dim < 256 && items <= 512 ? 2 : 1;
     s.blocks = s.splits > 1 && items < fill ? fill : items;
     s.records = s.splits > 1 ? fill : 0;
     s.joined = items < fill / 2 ? items : fill / 2;

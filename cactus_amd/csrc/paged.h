@@ -78,7 +78,7 @@ struct TileShape {
     int slots, splits, groups;
     size_t blocks, records, joined;
 };
-TileShape tile_shape(size_t head_dim, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
+TileShape tile_shape(size_t head_dim, bool paged, size_t batch, size_t tokens, size_t max_context, size_t q_heads, size_t kv_heads,
                      size_t window, size_t sink, bool beside);
 size_t tile_record_floats(size_t head_dim);
 hipError_t launch_attention_tiles(int head_dim, bool paged, const PagedAttnArgs& a, const TileShape& s, hipStream_t st);

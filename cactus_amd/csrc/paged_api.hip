@@ -120,7 +120,7 @@ PagedPlan paged_plan(const cactus_hip_paged_kv& c, size_t batch, size_t tokens, 
         if (p.step.splits > 1) p.step_bytes = p.step_items * p.step.rows * (c.head_dim + 2) * sizeof(float);
     }
     if (p.by_tile) {
-        p.tile = tile_shape(c.head_dim, batch, tokens, max_context, q_heads, c.kv_heads, window, sink, p.by_step);
+        p.tile = tile_shape(c.head_dim, true, batch, tokens, max_context, q_heads, c.kv_heads, window, sink, p.by_step);
         p.tile_items = p.tile.blocks;
         p.tile_bytes = p.tile.records * tile_record_floats(c.head_dim) * sizeof(float);
     }
@@ -297,7 +297,7 @@ int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride,
     a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)head_dim) : scale;
     a.window = reach(window);
     a.sink = reach(sink);
-    const TileShape s = tile_shape(head_dim, batch, tokens, 0, num_q_heads, num_kv_heads, window, sink, false);      // 0: never split
+    const TileShape s = tile_shape(head_dim, false, batch, tokens, 0, num_q_heads, num_kv_heads, window, sink, false);
     if (s.blocks >= MAX_ITEMS) return refuse(who, too_many);
     return launched(who, launch_attention_tiles((int)head_dim, false, a, s, (hipStream_t)stream));
 }

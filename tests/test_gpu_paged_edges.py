@@ -5,6 +5,7 @@ import math
 import pytest
 
 from tests import paged_reference as R
+from tests.test_gpu_paged import check_append, check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -180,3 +181,12 @@ def test_a_scale_that_is_not_positive_and_finite_counts_as_zero(P, D, which, bad
 
     for a, b in zip(results(bad), results(0.0)):
         assert bool(torch.isfinite(a).all()) and bool((a == b).all())
+
+
+# ------------------------------------------------------------------------------------------- hints, many pages, many sequences
+
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 32), (256, 64)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (300, 4)])
+def test_the_bound_of_a_chunk_batch_is_only_a_hint(P, D, page, window, sink):
+    for hint in (0, 127, 1 << 30):
+        check_attention(P, 3, D, page, 4, 2, [70, 0, 130, 1], [900, 3, 1301, 40], window, sink, max_context=hint)

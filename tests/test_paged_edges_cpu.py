@@ -1,6 +1,7 @@
 """CPU tests of the paged cache's boundary: calls that are almost empty, workspaces (the host decides
 both before anything is enqueued)."""
 import ctypes as C
+import re
 
 import pytest
 
@@ -29,3 +30,10 @@ def test_chunks_of_more_than_1024_sequences_need_no_workspace(dim, context):
     assert need(1025) == 0 and need(1 << 16) == 0
     # three sequences: two splits of the least number of keys, 256 at head_dim 64 and 128 above
     assert (need(3) > 0) == (context >= 2 * (256 if dim == 64 else 128))
+
+
+def test_two_groups_of_waves_are_for_fp16_prompts_only():
+    """max_context 0 is a legal bound over pages, and no sign of FP16 prompts: no kernel over pages has two groups."""
+    names = set(re.findall(rb"attention_tile_kernelILi(\d+)ELb([01])ELi([12])E", open(H.SO_PATH, "rb").read()))
+    assert names == {(d, p, g) for d in (b"64", b"128", b"256") for p in (b"0", b"1") for g in (b"1", b"2")
+                     if g == b"1" or (p == b"0" and d != b"256")}
