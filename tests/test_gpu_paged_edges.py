@@ -5,7 +5,7 @@ import math
 import pytest
 
 from tests import paged_reference as R
-from tests.test_gpu_paged import check_append, check_attention
+from tests.test_gpu_paged import check_append, check_attention, random_cache, read_back
 
 pytestmark = pytest.mark.gpu
 
@@ -190,3 +190,57 @@ def test_a_scale_that_is_not_positive_and_finite_counts_as_zero(P, D, which, bad
 def test_the_bound_of_a_chunk_batch_is_only_a_hint(P, D, page, window, sink):
     for hint in (0, 127, 1 << 30):
         check_attention(P, 3, D, page, 4, 2, [70, 0, 130, 1], [900, 3, 1301, 40], window, sink, max_context=hint)
+
+
+# How the launch cuts an append: workgroups for 1024 (page, items) pieces, all items of a page in one where there are as many
+# pages.  Pieces are floor(tokens / page) + 2 * sequences, at one row each one a sequence; a pass of a workgroup takes 256 or more
+# row slots of D / 16 lanes, so several items or query heads more than fit one need more passes.
+
+@pytest.mark.parametrize("D,page,Hq,Hkv,sequences", [(64, 16, 9, 3, 500), (64, 32, 6, 3, 520), (64, 64, 4, 2, 520), (128, 16, 3, 3, 500),
+                                                     (128, 64, 4, 2, 520), (256, 16, 2, 2, 500), (256, 128, 3, 1, 520)])
+def test_append_of_many_pages_in_several_passes(P, D, page, Hq, Hkv, sequences):
+    gen = torch.Generator().manual_seed(D + page)
+    news = [int(x) for x in torch.randint(0, 24, (sequences,), generator=gen)]
+    pasts = [int(x) for x in torch.randint(0, 3 * page, (sequences,), generator=gen)]
+    for b, n in ((0, 3 * page + 1), (70, 0), (200, 2 * page), (sequences - 1, page + 3)):
+        news[b] = n
+    pasts[300], pasts[301] = -1, -5
+    pieces = sum(news) // page + 2 * sequences
+    lanes = D // 16
+    slots = max(256, page * lanes if page * lanes <= 256 else page * lanes // 2) // lanes
+    assert pieces >= 1024 and 2 * Hkv > slots // min(page, slots) and Hq > slots // min(page, slots) // 2
+    check_append(P, 21, D, page, Hq, Hkv, news, pasts)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 80, 40), (128, 40, 20), (256, 18, 9)])
+def test_append_of_many_sequences_in_several_passes(P, D, Hq, Hkv):
+    gen = torch.Generator().manual_seed(D)
+    assert 2 * Hkv > 256 // (D // 16) and Hq > 256 // (D // 16)
+    pasts = [int(x) for x in torch.randint(0, 40, (1030,), generator=gen)]
+    pasts[3], pasts[1029] = -1, 16
+    check_append(P, 22, D, 16, Hq, Hkv, [1] * 1030, pasts, use_cu=False)
+
+
+def test_append_of_long_prompts_in_several_passes(P):
+    news, pasts = [1203, 1187, 1250, 1100, 1333, 1211, 1197], [0, 5, 31, 32, 33, 700, 0]
+    check_append(P, 23, 64, 32, 32, 8, news, pasts)
+
+
+@pytest.mark.parametrize("sequences", [64, 65, 66, 130, 200, 1000])
+def test_append_and_read_of_many_sequences(P, sequences):
+    """More sequences than a wave looks through at once, some of them without rows."""
+    gen = torch.Generator().manual_seed(sequences)
+    D, page, Hkv = 64, 16, 2
+    news = [int(x) for x in torch.randint(0, 5, (sequences,), generator=gen)]
+    pasts = [int(x) for x in torch.randint(0, 40, (sequences,), generator=gen)]
+    news[0], news[sequences // 2], news[sequences - 1] = 0, 50, 0
+    check_append(P, 24, D, page, 4, Hkv, news, pasts)
+    starts = [int(x) for x in torch.randint(0, 30, (sequences,), generator=gen)]
+    used = [(c + s + page - 1) // page for c, s in zip(news, starts)]
+    total = sum(used) + 2
+    tables = R.make_tables(gen, used, max(used), total)
+    kv = random_cache(gen, total, Hkv, page, D)
+    k, v = P.kv_read([x.cuda() for x in kv], tables.cuda(), i32(starts).cuda(), R.offsets(news).cuda(), sum(news))
+    want = [torch.cat([R.gather(x, y, tables[b], page, s, c)[0] for b, (c, s) in enumerate(zip(news, starts))])
+            for x, y in ((kv[0], kv[2]), (kv[1], kv[3]))]
+    assert read_back(k, want[0]) and read_back(v, want[1])
