@@ -3,7 +3,8 @@
 A cache is the tuple (k, v, k_scales, v_scales): int8 [num_pages, kv_heads, page_size, head_dim] twice and float32
 [num_pages, kv_heads] twice (empty_pages makes one).  block_tables int32 [batch, width] name the pages of each
 sequence, and rows of several sequences are packed one behind the other (cu_seqlens int32 [batch + 1]; None: one row
-each).  Every function enqueues on torch's current stream of the tensors' device and returns without synchronising.
+each).  Rows behind the last sequence (a padded batch) are not written: without an output tensor of the caller's they hold
+whatever the memory held.  Every function enqueues on torch's current stream of the tensors' device and returns without synchronising.
 """
 import ctypes as C
 
@@ -123,7 +124,8 @@ def kv_append(k, v, kv, block_tables, positions, theta, cu_seqlens=None, q=None,
               out_q=None):
     """Append the rows k / v fp16 [tokens, kv_heads, head_dim] of a step or prompt chunk to the cache at positions int32
     [batch] (tokens each sequence already has there; negative: the sequence is skipped), with per-head RMS norm (k_weight),
-    rotation (theta; 0: none) and quantization in one launch.  q fp16 [tokens, q_heads, head_dim], when given, is normed
+    rotation (theta; 0: none) and quantization in one launch.  A token that outgrows its page's scale raises it, and the page's
+    earlier codes are rounded once more (the header says what that costs).  q fp16 [tokens, q_heads, head_dim], when given, is normed
     (q_weight), rotated and returned."""
     c, dev, batch, width = _cache(kv, block_tables)
     tokens = k.shape[0]

@@ -244,3 +244,34 @@ def test_append_and_read_of_many_sequences(P, sequences):
     want = [torch.cat([R.gather(x, y, tables[b], page, s, c)[0] for b, (c, s) in enumerate(zip(news, starts))])
             for x, y in ((kv[0], kv[2]), (kv[1], kv[3]))]
     assert read_back(k, want[0]) and read_back(v, want[1])
+
+
+# ------------------------------------------------------------------------------------------- codes requantized many times
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("growth", ["normal", "spread", "slow"])
+def test_token_by_token_a_code_is_off_by_half_of_every_scale_it_had(P, page, growth):
+    """The cache against the FP16 rows themselves, over two pages filled a token at a time and in calls of five.  Each time a page's
+    scale grows its codes are rounded once more, by at most half a step of the new scale."""
+    gen = torch.Generator().manual_seed(page)
+    D, H, n = 128, 2, 2 * page
+    x = torch.randn((n, 2, H, D), generator=gen).clamp(-2.5, 2.5)
+    at = torch.arange(n).float().view(-1, 1, 1, 1)
+    x *= {"normal": 1 + 0 * at, "spread": torch.exp(0.5 * torch.randn((n, 1, 1, 1), generator=gen)), "slow": 1.004 ** at}[growth]
+    x = x.half()
+    t = i32([[1, 0]])
+    for step in (1, 5):
+        kv = P.empty_pages(2, H, D, page)
+        scales, bound = torch.zeros((2, 2, H), dtype=torch.float64), torch.zeros((2, 2, H), dtype=torch.float64)
+        for i in range(0, n, step):
+            m = min(step, n - i)
+            rows = x[i:i + m].cuda()
+            P.kv_append(rows[:, 0], rows[:, 1], kv, t.cuda(), i32([i]).cuda(), 0.0, cu_seqlens=i32([0, m]).cuda())
+            now = torch.stack([kv[2].cpu(), kv[3].cpu()]).double()
+            bound += torch.where(now > scales, 0.5 * now * (1 + 2 * 127 * 4 * R.U32), 0.0)
+            scales = now
+        back = [R.gather(kv[w].cpu(), kv[2 + w].cpu(), t[0], page, 0, n)[0] for w in range(2)]
+        for w in range(2):
+            for p in range(2):
+                err = (back[w][p * page:(p + 1) * page] - x[p * page:(p + 1) * page, w].double()).abs()
+                assert bool((err.amax((0, 2)) <= bound[w, int(t[0, p])]).all())
