@@ -75,6 +75,12 @@ const char* bad_groups(size_t q_heads, size_t kv_heads) {
     return nullptr;
 }
 
+// The kernels' running maximum starts at -1e30: rows of halves (and what append makes of them) have products of 1e14 at most, so
+// scores stay above that.
+const char* bad_scale(float scale) {
+    return std::fabs(scale) <= 1e15f ? nullptr : "scale must be finite, 1e15 at most";
+}
+
 const char* bad_window(size_t window, size_t sink) {
     return window > 0x7fffffff || sink > 0x7fffffff ? "window and sink must be below 2^31" : nullptr;
 }
@@ -232,7 +238,7 @@ int cactus_hip_attention_paged_f16_dev(const cactus_hip_paged_kv* cache, const i
     if (!context_lens) return refuse(who, "null context_lens");
     REFUSE_IF(bad_rows(q, q_stride, num_q_heads, cache->head_dim));
     REFUSE_IF(bad_rows(output, num_q_heads * cache->head_dim, num_q_heads, cache->head_dim));
-    if (!std::isfinite(scale)) return refuse(who, "scale must be finite");
+    REFUSE_IF(bad_scale(scale));
     PagedAttnArgs a{};
     a.c = view(*cache, block_tables, table_width);
     a.contexts = context_lens;
@@ -280,7 +286,7 @@ int cactus_hip_attention_ragged_f16_dev(const cactus_half_t* q, size_t q_stride,
     REFUSE_IF(bad_rows(k, k_stride, num_kv_heads, head_dim));
     REFUSE_IF(bad_rows(v, v_stride, num_kv_heads, head_dim));
     REFUSE_IF(bad_rows(output, num_q_heads * head_dim, num_q_heads, head_dim));
-    if (!std::isfinite(scale)) return refuse(who, "scale must be finite");
+    REFUSE_IF(bad_scale(scale));
     PagedAttnArgs a{};
     a.k = k;
     a.v = v;

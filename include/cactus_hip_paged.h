@@ -25,7 +25,7 @@
  *     window == 0   or   p - j <= window   or   j < sink
  * which is the sliding window of cactus_hip_attention_f16_dev (kernel_attention.cpp:81-87) plus `sink` leading tokens.  The
  * reference's KVCache window of W slots with S sink tokens (engine_cache.cpp:268-329) is window = W - S, sink = S.  A row
- * that sees nothing becomes zeros.  scale == 0 means 1 / sqrt(head_dim).
+ * that sees nothing becomes zeros.  scale == 0 means 1 / sqrt(head_dim); otherwise it is at most 1e15, of either sign.
  *
  * Calls enqueue on `stream`, allocate nothing, synchronize nothing and may be captured.  They use no library workspace:
  * scratch comes in as `workspace`, so calls on different streams do not meet.  Returns as in cactus_hip.h. */

@@ -37,3 +37,9 @@ def test_two_groups_of_waves_are_for_fp16_prompts_only():
     names = set(re.findall(rb"attention_tile_kernelILi(\d+)ELb([01])ELi([12])E", open(H.SO_PATH, "rb").read()))
     assert names == {(d, p, g) for d in (b"64", b"128", b"256") for p in (b"0", b"1") for g in (b"1", b"2")
                      if g == b"1" or (p == b"0" and d != b"256")}
+
+
+@pytest.mark.parametrize("call", [attend, ragged])
+@pytest.mark.parametrize("scale", [1e16, -1e16, 1e30, 3e38])
+def test_refuses_a_scale_whose_scores_leave_the_running_maximum_s_range(call, scale):
+    assert refused(call(scale=scale), "scale")
