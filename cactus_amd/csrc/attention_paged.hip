@@ -21,8 +21,9 @@
 // fp32 weights over s_v back.
 // The next block's rows are requested before the current one is computed (registers, two blocks deep).  The output is
 // rescaled only when a maximum has grown by more than 2^LAG.
-// Measured (16 heads over 8, D = 128): 256 sequences of 300 to 700 keys 50.1 us = 5.2 TB/s; 4 of 32k, 32 heads over 8, 45.8 us =
-// 5.6 TB/s and 4.6 for the join; one of 4096 5.8 + 3.4 us; 64 of window 508 + 4, 4 heads over 1, D = 256, 11.0 + 3.9 us.
+// Measured (16 heads over 8, D = 128; a read-only kernel reaches 6.75 TB/s): 256 sequences of 300 to 700 keys 50.8 us = 5.2 TB/s; 4 of
+// 32k, 32 heads over 8, 48.2 us with the join.  Kernels alone: 4 of 32k 45.7 us = 5.6 TB/s and 4.6 for the join; one of 4096 5.8 + 3.2
+// us; 64 of window 508 + 4, 4 heads over 1, D = 256, 11.0 + 3.9 us (13.4 in a row).
 #include "paged.hip.h"
 
 #include <math.h>

@@ -1,6 +1,7 @@
 // Attention of many query rows (include/cactus_hip_paged.h): packed FP16 prompts, and prompt chunks over the paged INT8
 // cache.  Bound: the matrix cores, the softmax's vector instructions and the LDS reads together, none of them alone: of the
-// 4800 cycles that two waves of a SIMD take for a key tile each (D = 128) the matrix cores work 2050.
+// 4800 cycles that two waves of a SIMD take for a key tile each (D = 128, in-kernel stamps) the matrix cores work 2050.  Over
+// a whole launch (prompt of 4096, counters) they are busy 33% of the cycles, vector instructions 31%, both at once 9%.
 //
 // A workgroup is four waves on 128 consecutive rows (64 at head_dim 256) of one (sequence, kv head); a row is (token, query head
 // of the group), so a key tile in LDS serves all query heads of its kv head.  A wave owns 32 rows (16) and computes everything
@@ -20,9 +21,9 @@
 // Weights are rounded to binary16 (2^-11 of each, averaged over the keys that count, down to 2^-25 of the largest: LIFT); everything
 // else is fp32.
 //
-// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 83 us, 829 TFLOP/s (a large FP16 matrix product reaches
-// 1139).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 87 us, 485.  24 prompts of 17 to 300 tokens,
-// D = 64: 17.3 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 43 us, 8 of them the join's.
+// Measured: one prompt of 4096 tokens, 16 heads over 8, D = 128: 84 us, 815 TFLOP/s (a large FP16 matrix product reaches
+// 1139 to 1334).  Prompts of 4001 to 8190 tokens, 4 heads over 1, D = 256, window 508: 88 us, 480.  24 prompts of 17 to 300 tokens,
+// D = 64: 18.0 us.  Three chunks of 131 to 256 tokens over 4000 cached ones: 44 us, 8 of them the join's.
 // Slower were: values stored transposed, one 16-byte read for two transposing 8-byte ones (99 and 60 us instead of 90 and 55 then:
 // turning them takes 8-byte loads, twice as many); two groups of waves half a tile apart instead of in step (101 instead of 97).
 #include "paged.hip.h"

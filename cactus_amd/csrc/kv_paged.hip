@@ -11,8 +11,8 @@
 // heads, otherwise tokens come first.  A lane keeps its tokens while it walks the heads, so an angle is computed once per
 // workgroup: in fp64 as turns (pos * theta^(-2i/D) / 2 pi, only the fraction kept), because an fp32 product at position 30000
 // is off by 1e-3; v_sin_f32 / v_cos_f32 take turns and are off by 2^-23 at most (measured).
-// Measured: 7 prompts of 500 to 1900 tokens, 32 + 2 x 8 heads of 64: 24 us = 4.5 TB/s (a large copy reaches 5.15); a step of one
-// sequence 4.7 us, of 256 6.4 us; 5 chunks of 100 to 256 tokens, 4 + 2 x 1 heads of 256 in pages of 128: 11.4 us, a chain of
+// Measured: 7 prompts of 500 to 1900 tokens, 32 + 2 x 8 heads of 64: 25 us = 4.5 TB/s (a large copy reaches 5.16); a step of one
+// sequence 4.9 us, of 256 6.8 us; 5 chunks of 100 to 256 tokens, 4 + 2 x 1 heads of 256 in pages of 128: 11.4 us, a chain of
 // row, maximum, store and requantization in 96 workgroups.
 #include "paged.hip.h"
 
