@@ -19,7 +19,7 @@
  * cu_seqlens[b + 1] - 1 of `tokens` (device int32 [batch + 1], not decreasing, starting at 0).  cu_seqlens == NULL: one row
  * per sequence (tokens == batch, a decode step).  Rows behind cu_seqlens[batch] are left as they are.  An input row is
  * half [heads][head_dim]; consecutive rows lie `stride` elements apart (a multiple of 8, at least heads * head_dim, below 2^24: q, k
- * and v may be columns of one fused projection); output rows are contiguous.
+ * and v may be columns of one fused projection); output rows are contiguous, and an output may be q itself where q's rows are too.
  *
  * Visibility, in every attention here: position p sees the keys j <= p of its sequence with
  *     window == 0   or   p - j <= window   or   j < sink

@@ -275,3 +275,28 @@ def test_token_by_token_a_code_is_off_by_half_of_every_scale_it_had(P, page, gro
             for p in range(2):
                 err = (back[w][p * page:(p + 1) * page] - x[p * page:(p + 1) * page, w].double()).abs()
                 assert bool((err.amax((0, 2)) <= bound[w, int(t[0, p])]).all())
+
+
+# ------------------------------------------------------------------------------------------- results in place of the queries
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("news,contexts", [([1] * 5, [1, 700, 64, 0, 300]), ([1], [5000]), ([70, 1, 0, 130], [900, 40, 3, 1301]), ([150], [150]),
+                                           ([3, 2, 40], [1000, 2, 2000])])
+def test_outputs_may_be_the_queries(P, D, news, contexts):
+    gen = torch.Generator().manual_seed(D)
+    page, Hq, Hkv, T = 32, 6, 2, sum(news)
+    used = [(c + page - 1) // page for c in contexts]
+    kv = [x.cuda() for x in random_cache(gen, sum(used) + 1, Hkv, page, D)]
+    t = R.make_tables(gen, used, max(used), sum(used) + 1).cuda()
+    cu = R.offsets(news).cuda()
+    ctx = i32(contexts).cuda()
+    q, k, v = (torch.randn((T, h, D), generator=gen).half().cuda() for h in (Hq, Hkv, Hkv))
+    past = ctx - (cu[1:] - cu[:-1])
+    calls = [lambda x, out: P.attention(x, kv, t, ctx, cu_seqlens=None if max(news) == 1 else cu, out=out),
+             lambda x, out: P.attention_ragged(x, k, v, cu, window=50, sink=3, out=out),
+             lambda x, out: P.kv_append(k, v, [y.clone() for y in kv], t, past, 1e4, cu_seqlens=cu, q=x, out_q=out)]
+    for call in calls:
+        own = q.clone()
+        want = call(q, q.clone())        # rows of a sequence that is skipped (a context of 0: position -1) stay as they were
+        assert call(own, own) is own
+        assert torch.equal(own, want)
